@@ -1,0 +1,283 @@
+// Rules on a row's logits before a token is chosen from it: penalties for tokens that are already there, biases on single
+// tokens, a mask of the tokens that may come.  For token v of a row whose request's text is h_0 .. h_(n-1), of which the first
+// p are its prompt, with c the number of v's among h_p .. h_(n-1):
+//   z1 = z / repetition if z > 0, else z * repetition,  where v occurs in the text, else z
+//   z2 = (z1 - frequency * c) - presence                where c > 0, else z1
+//   z3 = z2 + the row's bias of v (the last one listed, where v is listed more than once)
+//   z4 = z3 where the row's mask has bit v set (or the row has no mask), else -infinity, whatever z3 is
+// every operation rounded by itself in 32 bits.  adjust: z4 itself; choose: what sampling.hip chooses from z4, bit for bit,
+// without z4 ever being in memory.
+//
+// A workgroup has a slice of one row's vocabulary.  It counts its slice's tokens in the LDS (one word a token: occurrences in the
+// output, and two bits for "in the text" and "has a bias"), by integer additions, whose order does not matter, then streams
+// the slice's logits past those words.  Every slice reads the row's whole text; it comes from the L2 for all slices but one.
+#include "launch.hpp"
+#include "sampling.hpp"
+#pragma clang fp contract(off)      // the formulas' roundings, one by one
+
+constexpr int RULE_THREADS = 256;
+constexpr uint32_t SEEN = 0x80000000u, BIASED = 0x40000000u, TIMES = 0x3FFFFFFFu;
+
+struct Rules {
+  const int* history;      // [slots, most] tokens by position, or null: no penalties
+  long history_ld;
+  int slots, most;
+  const int* slot;         // [rows] of history
+  const int* length;       // [rows] tokens of the text
+  const int* prompt;       // [rows] of these, the prompt's
+  const float* repetition; // [rows] each
+  const float* presence;
+  const float* frequency;
+  const int* bias_starts;  // [rows + 1] into the lists, or null: no biases
+  const int* bias_tokens;
+  const float* bias_values;
+  int biases;              // entries of the lists
+  const uint32_t* masks;   // [num_masks, mask_ld] bit v % 32 of word v / 32, or null: no masks
+  long mask_ld;
+  int num_masks;
+  const int* mask_row;     // [rows]; what is not an index of a mask: none
+};
+
+__device__ __forceinline__ int clamp_int(int x, int low, int high) { return x < low ? low : (x > high ? high : x); }
+
+struct RowRules {
+  float repetition, presence, frequency;
+  const float* bias_values;      // of the row's list
+  const int* bias_at;            // LDS: 1 + the place in that list, of tokens whose word has BIASED
+};
+
+__device__ __forceinline__ float apply_rules(float z, uint32_t w, int i, const RowRules& r) {
+  if (w == 0) return z;
+  if (w & SEEN) z = z > 0.f ? z / r.repetition : z * r.repetition;
+  const uint32_t c = w & TIMES;
+  if (c) {
+    z = z - r.frequency * (float)c;
+    z = z - r.presence;
+  }
+  if (w & BIASED) z = z + r.bias_values[r.bias_at[i] - 1];
+  return z;
+}
+
+// Grid (slices, rows).  CHOOSE: the slice's best candidate to best_v, best_i [rows, slices], or, of a row that is one slice, the
+// token to ``chosen``; else the adjusted logits to ``out``.  VEC: rows of logits (and of ``out``) begin on 16 bytes.
+template <bool CHOOSE, bool VEC>
+__global__ void __launch_bounds__(RULE_THREADS)
+rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float* out, long out_ld,
+             const float* __restrict__ temperatures, const long long* __restrict__ seeds, const int* __restrict__ counters,
+             float* __restrict__ best_v, int* __restrict__ best_i, int* __restrict__ chosen) {
+  extern __shared__ __align__(16) uint32_t words[];                   // [slice], then, with biases, [slice] places in the list
+  int* bias_at = reinterpret_cast<int*>(words + slice);
+  __shared__ float wave_v[RULE_THREADS / 64];
+  __shared__ int wave_i[RULE_THREADS / 64];
+  const int r = blockIdx.y, begin = blockIdx.x * slice, n = min(slice, V - begin);
+  const int tid = threadIdx.x;
+
+  RowRules row{1.f, 0.f, 0.f, nullptr, bias_at};
+  int length = 0, prompt = 0;
+  const int* text = nullptr;
+  if (rules.history) {
+    row.repetition = rules.repetition[r];
+    row.presence = rules.presence[r];
+    row.frequency = rules.frequency[r];
+    const int s = rules.slot[r];
+    if ((row.repetition != 1.f || row.presence != 0.f || row.frequency != 0.f) && s >= 0 && s < rules.slots) {
+      text = rules.history + (size_t)s * rules.history_ld;
+      length = clamp_int(rules.length[r], 0, rules.most);
+      prompt = clamp_int(rules.prompt[r], 0, length);
+    }
+  }
+  int listed = 0;
+  const int* list = nullptr;
+  if (rules.bias_starts) {
+    const int a = clamp_int(rules.bias_starts[r], 0, rules.biases), b = clamp_int(rules.bias_starts[r + 1], a, rules.biases);
+    listed = b - a;
+    list = rules.bias_tokens + a;
+    row.bias_values = rules.bias_values + a;
+  }
+  const uint32_t* mask = nullptr;
+  if (rules.masks) {
+    const int m = rules.mask_row[r];
+    if (m >= 0 && m < rules.num_masks) mask = rules.masks + (size_t)m * rules.mask_ld;
+  }
+  const bool counted = length > 0 || listed > 0;                      // (the same in the whole workgroup)
+  if (counted) {
+    for (int i = tid; i < n; i += RULE_THREADS) {
+      words[i] = 0;
+      if (listed > 0) bias_at[i] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < length; i += RULE_THREADS) {
+      const unsigned at = (unsigned)(text[i] - begin);                // what is no token of the vocabulary is in no slice
+      if (at < (unsigned)n) {
+        atomicOr(&words[at], SEEN);
+        if (i >= prompt) atomicAdd(&words[at], 1u);
+      }
+    }
+    for (int i = tid; i < listed; i += RULE_THREADS) {
+      const unsigned at = (unsigned)(list[i] - begin);
+      if (at < (unsigned)n) {
+        atomicOr(&words[at], BIASED);
+        atomicMax(&bias_at[at], i + 1);
+      }
+    }
+    __syncthreads();
+  }
+
+  const float* z0 = logits + (size_t)r * ld + begin;
+  float* o0 = CHOOSE ? nullptr : out + (size_t)r * out_ld + begin;
+  bool noisy = false;
+  float inv_t = 1.f;
+  uint32_t key = 0;
+  if (CHOOSE) {
+    const float t = temperatures[r];
+    noisy = t > 0.f;
+    if (noisy) {
+      inv_t = 1.0f / t;
+      key = sample_key((unsigned long long)seeds[r], counters[r]);
+    }
+  }
+  float bv = -INFINITY;
+  int bi = 0x7FFFFFFF;
+  const int n4 = VEC ? n & ~3 : 0;
+  for (int i = tid * 4; i < n4; i += RULE_THREADS * 4) {
+    const float4 z = *reinterpret_cast<const float4*>(z0 + i);
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (counted) w = *reinterpret_cast<const uint4*>(words + i);
+    const uint32_t bits = mask ? mask[(begin + i) >> 5] >> ((begin + i) & 31) : 15u;
+    float4 y;
+    y.x = bits & 1 ? apply_rules(z.x, w.x, i, row) : -INFINITY;
+    y.y = bits & 2 ? apply_rules(z.y, w.y, i + 1, row) : -INFINITY;
+    y.z = bits & 4 ? apply_rules(z.z, w.z, i + 2, row) : -INFINITY;
+    y.w = bits & 8 ? apply_rules(z.w, w.w, i + 3, row) : -INFINITY;
+    if (CHOOSE) {
+      sample_consider(y.x, begin + i, noisy, inv_t, key, bv, bi);
+      sample_consider(y.y, begin + i + 1, noisy, inv_t, key, bv, bi);
+      sample_consider(y.z, begin + i + 2, noisy, inv_t, key, bv, bi);
+      sample_consider(y.w, begin + i + 3, noisy, inv_t, key, bv, bi);
+    } else {
+      *reinterpret_cast<float4*>(o0 + i) = y;
+    }
+  }
+  for (int i = n4 + tid; i < n; i += RULE_THREADS) {
+    const bool may = !mask || (mask[(begin + i) >> 5] >> ((begin + i) & 31) & 1);
+    const float z = z0[i];
+    const float y = may ? apply_rules(z, counted ? words[i] : 0, i, row) : -INFINITY;
+    if (CHOOSE) sample_consider(y, begin + i, noisy, inv_t, key, bv, bi);
+    else o0[i] = y;
+  }
+  if (!CHOOSE) return;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float ov = __shfl_xor(bv, o, 64);
+    const int oi = __shfl_xor(bi, o, 64);
+    sample_better(ov, oi, bv, bi);
+  }
+  if ((tid & 63) == 0) { wave_v[tid >> 6] = bv; wave_i[tid >> 6] = bi; }
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < RULE_THREADS / 64; ++i) sample_better(wave_v[i], wave_i[i], bv, bi);
+    if (gridDim.x == 1) {
+      chosen[r] = bi == 0x7FFFFFFF ? 0 : bi;
+    } else {
+      best_v[(size_t)r * gridDim.x + blockIdx.x] = bv;
+      best_i[(size_t)r * gridDim.x + blockIdx.x] = bi;
+    }
+  }
+}
+
+// The best of a row's slices, one wave a row.
+__global__ void __launch_bounds__(64)
+best_of_slices_kernel(const float* __restrict__ best_v, const int* __restrict__ best_i, int* __restrict__ chosen, int slices) {
+  const size_t r = blockIdx.x;
+  float bv = -INFINITY;
+  int bi = 0x7FFFFFFF;
+  for (int i = threadIdx.x; i < slices; i += 64) sample_better(best_v[r * slices + i], best_i[r * slices + i], bv, bi);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float ov = __shfl_xor(bv, o, 64);
+    const int oi = __shfl_xor(bi, o, 64);
+    sample_better(ov, oi, bv, bi);
+  }
+  if (threadIdx.x == 0) chosen[r] = bi == 0x7FFFFFFF ? 0 : bi;
+}
+
+// history[slot of the token's row, its position] = the token, of every token of a step.
+__global__ void __launch_bounds__(256)
+record_tokens_kernel(int* __restrict__ history, long ld, int slots, int most, const int* __restrict__ ids, const int* __restrict__ taken_from,
+                     const int* __restrict__ earlier, int num_earlier, const int* __restrict__ token_row, const int* __restrict__ state_slots,
+                     int rows, const int* __restrict__ positions, int T) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= T) return;
+  const int r = token_row[t], p = positions[t], from = taken_from ? taken_from[t] : -1;
+  if (r < 0 || r >= rows || p < 0 || p >= most) return;
+  const int s = state_slots[r];
+  if (s < 0 || s >= slots) return;
+  history[(size_t)s * ld + p] = from >= 0 && from < num_earlier ? earlier[from] : ids[t];
+}
+
+MIE_EXPORT const char* logit_rules_last_error() { return g_mie_error; }
+
+// Tokens of the vocabulary that a workgroup takes.
+MIE_EXPORT int mie_rules_slice(int rows, int V) {
+  int slice = 1024;
+  while (slice < 4096 && (long)rows * ((V + slice - 1) / slice) > 4L * mie_compute_units()) slice *= 2;
+  return slice;
+}
+
+static int check_rules(const char* what, const Rules& r, int rows, int V, long ld) {
+  if (V <= 0 || ld < V) MIE_FAIL("%s: vocabulary %d, leading dim %ld", what, V, ld);
+  if (rows > 65535) MIE_FAIL("%s: %d rows, at most 65535", what, rows);
+  if (r.history && (r.most < 0 || r.history_ld < r.most || r.slots < 0)) MIE_FAIL("%s: history of %d slots, %d positions, %ld apart", what, r.slots, r.most, r.history_ld);
+  if (r.masks && (r.mask_ld < (V + 31) / 32 || r.num_masks < 0)) MIE_FAIL("%s: masks of %ld words for a vocabulary of %d", what, r.mask_ld, V);
+  return 0;
+}
+
+template <bool CHOOSE>
+static int launch_rules(const char* what, const float* logits, long ld, const Rules& rules, int rows, int V, float* out, long out_ld,
+                        const float* temperatures, const long long* seeds, const int* counters, float* best_v, int* best_i, int* chosen,
+                        hipStream_t stream) {
+  if (rows <= 0) return 0;
+  if (check_rules(what, rules, rows, V, ld)) return -1;
+  const int slice = mie_rules_slice(rows, V), slices = (V + slice - 1) / slice;
+  const int lds = slice * 4 * (rules.bias_starts ? 2 : 1);
+  const bool vec = ((uintptr_t)logits & 15) == 0 && (ld & 3) == 0 && (CHOOSE || (((uintptr_t)out & 15) == 0 && (out_ld & 3) == 0));
+  auto* kernel = vec ? rules_kernel<CHOOSE, true> : rules_kernel<CHOOSE, false>;
+  hipLaunchKernelGGL(kernel, dim3(slices, rows), dim3(RULE_THREADS), lds, stream, logits, ld, rules, V, slice, out, out_ld, temperatures,
+                     seeds, counters, best_v, best_i, chosen);
+  MIE_CHECK_LAUNCH(what);
+  if (CHOOSE && slices > 1) {
+    hipLaunchKernelGGL(best_of_slices_kernel, dim3(rows), dim3(64), 0, stream, best_v, best_i, chosen, slices);
+    MIE_CHECK_LAUNCH(what);
+  }
+  return 0;
+}
+
+#define RULE_ARGS                                                                                                                    \
+  const int *history, long history_ld, int slots, int most, const int *slot, const int *length, const int *prompt,                    \
+      const float *repetition, const float *presence, const float *frequency, const int *bias_starts, const int *bias_tokens,         \
+      const float *bias_values, int biases, const uint32_t *masks, long mask_ld, int num_masks, const int *mask_row
+#define RULES                                                                                                                         \
+  Rules { history, history_ld, slots, most, slot, length, prompt, repetition, presence, frequency, bias_starts, bias_tokens,          \
+          bias_values, biases, masks, mask_ld, num_masks, mask_row }
+
+MIE_EXPORT int mie_adjust_logits(const float* logits, long ld, RULE_ARGS, float* out, long out_ld, int rows, int V, hipStream_t stream) {
+  if (rows > 0 && out_ld < V) MIE_FAIL("adjust_logits: rows of the result %ld apart for a vocabulary of %d", out_ld, V);
+  return launch_rules<false>("adjust_logits", logits, ld, RULES, rows, V, out, out_ld, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, stream);
+}
+
+// best_v, best_i: [rows, slices of mie_rules_slice] (unused where that is one)
+MIE_EXPORT int mie_choose_by_rules(const float* logits, long ld, RULE_ARGS, const float* temperatures, const long long* seeds,
+                                   const int* counters, float* best_v, int* best_i, int* chosen, int rows, int V, hipStream_t stream) {
+  return launch_rules<true>("sample", logits, ld, RULES, rows, V, nullptr, 0, temperatures, seeds, counters, best_v, best_i, chosen, stream);
+}
+
+MIE_EXPORT int mie_record_tokens(int* history, long ld, int slots, int most, const int* ids, const int* taken_from, const int* earlier,
+                                 int num_earlier, const int* token_row, const int* state_slots, int rows, const int* positions, int T,
+                                 hipStream_t stream) {
+  if (T <= 0) return 0;
+  if (ld < most) MIE_FAIL("record_tokens: history of %d positions, %ld apart", most, ld);
+  hipLaunchKernelGGL(record_tokens_kernel, dim3((T + 255) / 256), dim3(256), 0, stream, history, ld, slots, most, ids, taken_from, earlier,
+                     num_earlier, token_row, state_slots, rows, positions, T);
+  MIE_CHECK_LAUNCH("record_tokens");
+  return 0;
+}

@@ -9,28 +9,9 @@
 //   x_v = fmix(key ^ fmix(v + 0x9E3779B9));   u_v = ((x_v >> 9) + 0.5) * 2^-23
 // so the draw for (seed, counter) is the same in any batch.  Greedy and sampled rows share the
 // kernel; nothing is decided on the host.
-#include "common.hpp"
-
-__device__ __forceinline__ uint32_t fmix32(uint32_t x) {
-  x ^= x >> 16;
-  x *= 0x85EBCA6Bu;
-  x ^= x >> 13;
-  x *= 0xC2B2AE35u;
-  x ^= x >> 16;
-  return x;
-}
+#include "sampling.hpp"
 
 #define SAMPLE_THREADS 1024
-
-// One candidate: its value after temperature and noise, kept if it beats the best so far.
-__device__ __forceinline__ void sample_consider(float z, int v, bool noisy, float inv_t, uint32_t key, float& bv, int& bi) {
-  if (noisy) {
-    const uint32_t x = fmix32(key ^ fmix32((uint32_t)v + 0x9E3779B9u));
-    const float u = ((float)(x >> 9) + 0.5f) * 1.1920928955078125e-07f;   // 2^-23
-    z = z * inv_t - logf(-logf(u));
-  }
-  if (z > bv || (z == bv && v < bi)) { bv = z; bi = v; }
-}
 
 // VEC: the row is read four values at a time (needs a 16-byte aligned row), several reads in flight a thread.
 template <bool VEC>
@@ -45,10 +26,7 @@ sample_kernel(const float* __restrict__ logits, long ld, const float* __restrict
   const bool noisy = temp > 0.f;
   const float inv_t = noisy ? 1.0f / temp : 1.0f;
   uint32_t key = 0;
-  if (noisy) {
-    const unsigned long long seed = (unsigned long long)seeds[r];
-    key = fmix32(fmix32(fmix32((uint32_t)seed) ^ (uint32_t)(seed >> 32)) ^ (uint32_t)counters[r]);
-  }
+  if (noisy) key = sample_key((unsigned long long)seeds[r], counters[r]);
   float bv = -INFINITY;
   int bi = 0x7FFFFFFF;
   if (VEC) {
@@ -71,14 +49,13 @@ sample_kernel(const float* __restrict__ logits, long ld, const float* __restrict
   for (int o = 32; o > 0; o >>= 1) {
     const float ov = __shfl_xor(bv, o, 64);
     const int oi = __shfl_xor(bi, o, 64);
-    if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
+    sample_better(ov, oi, bv, bi);
   }
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if (lane == 0) { best_v[w] = bv; best_i[w] = bi; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < SAMPLE_THREADS / 64; ++i)
-      if (best_v[i] > bv || (best_v[i] == bv && best_i[i] < bi)) { bv = best_v[i]; bi = best_i[i]; }
+    for (int i = 1; i < SAMPLE_THREADS / 64; ++i) sample_better(best_v[i], best_i[i], bv, bi);
     out[r] = bi == 0x7FFFFFFF ? 0 : bi;
   }
 }

@@ -115,6 +115,37 @@ class StreamCopy:
         self.stream, self.value = stream, value
 
 
+@dataclass
+class LogitRules:
+    """What a row's request asks of its logits before a token is chosen, for R rows of logits over a vocabulary of V (tensors on the
+    device; each of the three groups may be left out).
+
+    Penalties: row r's text is the first ``lengths[r]`` numbers of ``history[slots[r]]`` (``history`` int32 [slots, positions], rows may
+    be further apart; numbers that are no token of the vocabulary count for nothing), its first ``prompt_lengths[r]`` the prompt.  A
+    token that occurs in the text has its logit divided (above 0) or multiplied by ``repetition[r]`` (> 0; 1: none); one that occurs
+    c > 0 times behind the prompt loses ``frequency[r]`` * c and then ``presence[r]``.  Index arrays int32 [R], penalties float32 [R].
+    A slot outside the history has no text.
+
+    Biases: ``bias_values[i]`` is added to the logit of token ``bias_tokens[i]``, i from ``bias_starts[r]`` up to ``bias_starts[r + 1]``
+    (int32 [R + 1]); of a token listed more than once in a row the last one counts.
+
+    Masks: ``masks`` int32 [masks, >= ceil(V / 32)]: token v may come if bit v % 32 of word v // 32 of row ``mask_rows[r]`` is set; a
+    mask row of -1 (or any number that is no index of a mask) is no mask.  What may not come has -infinity, whatever its logit (or NaN)
+    was."""
+    history: Any = None
+    slots: Any = None
+    lengths: Any = None
+    prompt_lengths: Any = None
+    repetition: Any = None
+    presence: Any = None
+    frequency: Any = None
+    bias_starts: Any = None
+    bias_tokens: Any = None
+    bias_values: Any = None
+    masks: Any = None
+    mask_rows: Any = None
+
+
 class KernelBackend:
     name = "?"
     act_dtype = None
@@ -441,7 +472,20 @@ class KernelBackend:
         Returns [T, Hq * D] in act_dtype."""
         raise NotImplementedError
 
-    def sample(self, logits, temperatures, seeds, counters, out=None):
+    def sample(self, logits, temperatures, seeds, counters, out=None, rules=None):
         """Per row: argmax(logits) if temperature == 0, else argmax(logits / temperature + g)
-        with Gumbel noise g from (seed, counter, vocabulary index).  -> [R] int32 (``out`` if given)."""
+        with Gumbel noise g from (seed, counter, vocabulary index).  -> [R] int32 (``out`` if given).  The lowest index among
+        equals; NaN is never chosen, and a row without a number (all NaN, or a mask that lets nothing through) gives token 0.
+        With ``rules`` (LogitRules) of what ``adjust_logits`` makes of the logits, which stay as they are."""
+        raise NotImplementedError
+
+    def adjust_logits(self, logits, rules, out=None):
+        """logits [R, V] float32 under ``rules`` (LogitRules): penalties, then biases, then masks, each operation rounded by itself
+        -> [R, V] float32, into ``out`` (which may be the logits themselves; rows may be further apart) or a new tensor."""
+        raise NotImplementedError
+
+    def record_tokens(self, history, step):
+        """history[step.state_slots[row of t], step.positions[t]] = token t of the step, for every token (what the step before chose
+        where step.taken_from says so): what LogitRules reads as a request's text.  history int32 [slots, positions]; tokens beyond
+        its slots or positions are left out."""
         raise NotImplementedError

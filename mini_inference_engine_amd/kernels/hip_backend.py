@@ -1972,11 +1972,54 @@ class HipBackend(KernelBackend):
                                                               int(getattr(step, "max_context", 0) or 0), self._stream()))
         return True
 
-    def sample(self, logits, temperatures, seeds, counters, out=None):
-        self._on_device(logits, temperatures, seeds, counters, out)
+    def _check_logits(self, what, logits):
         if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
-            raise ValueError("sample: logits must be float32 [rows, vocab] with unit inner stride")
-        R, V = logits.shape
+            raise ValueError(f"{what}: logits must be float32 [rows, vocab] with unit inner stride")
+        return logits.shape
+
+    def _rules_arguments(self, what, rules, R, V):
+        """What the kernels of csrc/logit_rules.hip take of a LogitRules, checked."""
+        dev = self._device_index
+
+        def vector(name, dtype, n=R):
+            t = getattr(rules, name)
+            if t is None:
+                raise ValueError(f"{what}: rules without {name}")
+            if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.stride(0) != 1 and n > 1 or t.get_device() != dev:
+                raise ValueError(f"{what}: rules.{name} must be contiguous {dtype} [{n}] on this GPU")
+            return t.data_ptr()
+
+        def table(name):
+            t = getattr(rules, name)
+            if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1 or t.get_device() != dev:
+                raise ValueError(f"{what}: rules.{name} must be int32 with unit inner stride, of two dimensions, on this GPU")
+            if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+                raise ValueError(f"{what}: rules.{name} has rows that overlap")
+            return t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[0], t.shape[1]
+
+        i32, f32 = torch.int32, torch.float32
+        args = [None, 0, 0, 0, None, None, None, None, None, None, None, None, None, 0, None, 0, 0, None]
+        if rules.history is not None:
+            args[0:4] = table("history")
+            args[4:10] = (vector("slots", i32), vector("lengths", i32), vector("prompt_lengths", i32), vector("repetition", f32),
+                          vector("presence", f32), vector("frequency", f32))
+            if args[0] == 0:        # a history without numbers: nobody has a text
+                args[0] = None
+        if rules.bias_starts is not None:
+            n = rules.bias_tokens.shape[0] if rules.bias_tokens is not None else 0
+            args[10:14] = vector("bias_starts", i32, R + 1), vector("bias_tokens", i32, n), vector("bias_values", f32, n), n
+        if rules.masks is not None:
+            at, ld, masks, words = table("masks")
+            if words < (V + 31) // 32:
+                raise ValueError(f"{what}: masks of {words} words for a vocabulary of {V}")
+            args[14:18] = at, ld, masks, vector("mask_rows", i32)
+            if masks == 0:
+                args[14] = None
+        return args
+
+    def sample(self, logits, temperatures, seeds, counters, out=None, rules=None):
+        self._on_device(logits, temperatures, seeds, counters, out)
+        R, V = self._check_logits("sample", logits)
         if (temperatures.dtype, seeds.dtype, counters.dtype) != (torch.float32, torch.int64, torch.int32):
             raise ValueError("sample: temperatures float32, seeds int64, counters int32")
         if not (temperatures.shape[0] == seeds.shape[0] == counters.shape[0] == R):
@@ -1985,7 +2028,58 @@ class HipBackend(KernelBackend):
             out = torch.empty(R, dtype=torch.int32, device=logits.device)
         elif out.dtype != torch.int32 or tuple(out.shape) != (R,) or not out.is_contiguous():
             raise ValueError(f"sample: out must be contiguous int32 [{R}]")
+        if rules is not None:
+            return self._choose_by_rules(logits, temperatures, seeds, counters, out, rules, R, V)
         lib = self.lib("sampling")
         library.check(lib, lib.mie_sample(_ptr(logits), logits.stride(0), _ptr(temperatures), _ptr(seeds),
                                           _ptr(counters), _ptr(out), R, V, self._stream()))
         return out
+
+    def _choose_by_rules(self, logits, temperatures, seeds, counters, out, rules, R, V):
+        if not (temperatures.is_contiguous() and seeds.is_contiguous() and counters.is_contiguous()):
+            raise ValueError("sample: temperatures, seeds and counters must be contiguous")
+        args = self._rules_arguments("sample", rules, R, V)
+        lib = self.lib("logit_rules")
+        slices = -(-V // lib.mie_rules_slice(R, V)) if V else 1
+        best = torch.empty((2, R, slices), dtype=torch.int32, device=logits.device) if slices > 1 else None
+        at = best.data_ptr() if best is not None else None
+        library.check(lib, lib.mie_choose_by_rules(
+            logits.data_ptr(), max(logits.stride(0), V), *args, temperatures.data_ptr(), seeds.data_ptr(), counters.data_ptr(), at,
+            None if at is None else at + 4 * R * slices, out.data_ptr(), R, V, self._stream()))
+        return out
+
+    def adjust_logits(self, logits, rules, out=None):
+        self._on_device(logits, out)
+        R, V = self._check_logits("adjust_logits", logits)
+        if out is None:
+            out = torch.empty((R, V), dtype=torch.float32, device=logits.device)
+        elif out.dtype != torch.float32 or tuple(out.shape) != (R, V) or out.stride(1) != 1 or (R > 1 and out.stride(0) < V):
+            raise ValueError(f"adjust_logits: out must be float32 [{R}, {V}] with unit inner stride and rows that do not overlap")
+        if R and (out.data_ptr(), out.stride(0)) != (logits.data_ptr(), logits.stride(0)):
+            span = lambda t: (t.data_ptr(), t.data_ptr() + ((R - 1) * t.stride(0) + V) * 4)     # noqa: E731
+            (a, b), (c, d) = span(out), span(logits)
+            if a < d and c < b:
+                raise ValueError("adjust_logits: out is the logits themselves or apart from them")
+        args = self._rules_arguments("adjust_logits", rules, R, V)
+        lib = self.lib("logit_rules")
+        library.check(lib, lib.mie_adjust_logits(logits.data_ptr(), max(logits.stride(0), V), *args, out.data_ptr(), max(out.stride(0), V),
+                                                 R, V, self._stream()))
+        return out
+
+    def record_tokens(self, history, step):
+        T, rows = step.num_tokens, step.num_rows
+        self._on_device(history, step.input_ids, step.taken_from, step.earlier_tokens, step.token_row, step.state_slots, step.positions)
+        if history.dtype != torch.int32 or history.dim() != 2 or history.stride(1) != 1 or history.stride(0) < history.shape[1]:
+            raise ValueError("record_tokens: history must be int32 [slots, positions] with unit inner stride and rows that do not overlap")
+        for name, t, n in (("input_ids", step.input_ids, T), ("token_row", step.token_row, T), ("positions", step.positions, T),
+                           ("state_slots", step.state_slots, rows), ("taken_from", step.taken_from, T), ("earlier_tokens", step.earlier_tokens, 0)):
+            if t is None and name in ("taken_from", "earlier_tokens"):
+                continue
+            if t is None or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
+                raise ValueError(f"record_tokens: {name} must be contiguous int32 [{n}]")
+        earlier = step.earlier_tokens if step.taken_from is not None else None
+        lib = self.lib("logit_rules")
+        library.check(lib, lib.mie_record_tokens(
+            _ptr(history), history.stride(0), history.shape[0], history.shape[1], _ptr(step.input_ids),
+            _ptr(step.taken_from if earlier is not None else None), _ptr(earlier), 0 if earlier is None else earlier.shape[0],
+            _ptr(step.token_row), _ptr(step.state_slots), rows, _ptr(step.positions), T, self._stream()))

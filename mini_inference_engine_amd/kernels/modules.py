@@ -117,6 +117,13 @@ register_kernel_module("attention", {
 register_kernel_module("sampling", {
     "mie_sample": [P, L, P, P, P, P, I, I, P],
 })
+_rules = [P, L, I, I, P, P, P, P, P, P, P, P, P, I, P, L, I, P]
+register_kernel_module("logit_rules", {
+    "mie_rules_slice": [I, I],
+    "mie_adjust_logits": [P, L, *_rules, P, L, I, I, P],
+    "mie_choose_by_rules": [P, L, *_rules, P, P, P, P, P, P, I, I, P],
+    "mie_record_tokens": [P, L, I, I, P, P, P, I, P, P, I, P, I, P],
+})
 register_kernel_module("gemm_bf16", {
     "mie_skinny_tiles": [I, I, I],
     "mie_skinny_held": [I, I, I, I],
