@@ -1,0 +1,453 @@
+// Attention of single-token rows whose requests share the first part of their cache, the shared keys read once for all of them.
+// Caches: keys [pages, Hkv, page, D], values [pages, Hkv, D, page], bfloat16 or float32.
+//
+// softmax(s q . k) v splits over any cut of the keys: with m a running maximum, l = sum exp2(x - m) and o = sum exp2(x - m) v of
+// each part, parts join by their log-sum-exps m + log2 l.  A plan made on the host (kernels/shared_prefix.py) cuts a step into
+// items: columns x keys of one kv head.  A column is one query head of one row; the columns of an item over shared keys are the
+// group's query heads of up to 64 CT / G rows (G query heads a kv head), those of an item over a row's own keys are its G query heads.
+// One workgroup an item and kv head: its four waves bring the keys and values of 32 keys after 32 into the LDS by loads that write the
+// LDS directly, NST - 1 blocks ahead, and each wave takes 16 CT of the columns through all of them:
+//   S^T[key, column]  = K[key, d] . Q^T[d, column]        A = 16 keys, B = 16 columns (16x16x32 bfloat16, 16x16x4 float32)
+//   O^T[dim, column] += V^T[dim, key] . P^T[key, column]
+// The scores come out with lane % 16 = column and 4 consecutive rows a lane group.  In bfloat16 the 32 keys are dealt to the two score
+// tiles' rows so that lane group g ends up with keys 8 g .. 8 g + 7, which is what the second product takes of both operands; in float32 every
+// one of the second product's steps of 4 keys takes one number of each lane group.  Probabilities never leave registers.
+#include "attention_bf16_common.hpp"
+#include "launch.hpp"
+
+constexpr int WAVES = 4;
+
+// 16 bytes a lane from a lane's own address into the LDS at byte `at` + 16 lane (waits are the kernel's own)
+__device__ __forceinline__ void lane_load_to_lds(const char* from, uint32_t at) {
+  uint32_t written;
+  asm volatile(
+    "s_mov_b32 m0, %1\n\t"
+    "s_nop 0\n\t"
+    "global_load_lds_dwordx4 %2, off"
+    : "={m0}"(written)
+    : "s"(at), "v"(from)
+    : "memory");
+}
+
+struct SharedItem {
+  int first_row;      // whose block table finds the keys
+  int columns;        // of the item's rows: rows x G
+  int col0;           // first of them that the item takes
+  int key_begin, key_end;
+  int part;           // which of its rows' partial results
+  int unused0, unused1;
+};
+
+template <typename T> struct Kind;
+template <> struct Kind<bf16> {
+  static constexpr int STAGES = D <= 32 ? 6 : D <= 64 ? 4 : 3;
+};
+template <> struct Kind<float> {
+  static constexpr int STAGES = D <= 64 ? 4 : D <= 128 ? 3 : 2;
+};
+
+template <typename T>
+struct Layout {
+  static constexpr int ES = sizeof(T);
+  static constexpr int ROW = D * ES;                        // bytes of a key
+  static constexpr int CHUNKS = ROW / 16;
+  static constexpr int TURN = CHUNKS % 8 == 0 ? 7 : CHUNKS % 4 == 0 ? 3 : 1;
+  static constexpr int VROW = 16 * ES;                      // bytes of 16 keys' values of one dim
+  static constexpr int TILE = 32 * ROW;                     // keys of a block; values take as much
+  static constexpr int UNITS = 2 * TILE / 1024;             // of a block's loads
+  static constexpr int EACH = (UNITS + WAVES - 1) / WAVES;  // a wave's
+  static constexpr int STAGES = Kind<T>::STAGES;
+  static constexpr int LDS = STAGES * 2 * TILE;
+  // 16-byte places are turned by what tells the rows apart that are read at once, so that they lie in different banks
+  static __device__ __forceinline__ int key_turn(int r) { return (ES == 2 ? (r & 3) | ((r >> 3 & 1) << 2) : r & 7) & TURN; }
+  static __device__ __forceinline__ int value_turn(int d) { return ES == 2 ? d >> 2 & 1 : d >> 1 & 3; }
+};
+
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ bf16 load_one(const bf16* p) { return *p; }
+
+template <typename T, int CT>
+__global__ void __launch_bounds__(WAVES * 64)
+shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
+                        T* __restrict__ out, float* __restrict__ o_part, float* __restrict__ lse_part, const int* __restrict__ tables,
+                        int max_blocks, int pages, const int* __restrict__ positions, const SharedItem* __restrict__ items,
+                        const int* __restrict__ row_parts, int Hq, int Hkv, int page, float scale_log2, float sink_log2,
+                        const float* __restrict__ head_sinks) {
+  using L = Layout<T>;
+  constexpr bool HALF = sizeof(T) == 2;
+  constexpr int QS = HALF ? KS : D / 16;                    // 16-byte pieces of a column's query that a lane holds
+  extern __shared__ __align__(1024) char lds[];
+  const int item = blockIdx.x / Hkv, kvh = blockIdx.x - item * Hkv;
+  const int first_row = items[item].first_row, columns = items[item].columns, col0 = items[item].col0;
+  const int key_begin = items[item].key_begin, part = items[item].part;
+  int key_end = items[item].key_end;
+  const int G = Hq / Hkv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kb = lane >> 4;
+  if (columns <= G) {                                       // one row: nothing behind its own key
+    const int seen = positions[first_row] + 1;
+    key_end = seen < key_end ? seen : key_end;
+  }
+
+  // ---- the loads: unit u of a block is 1 KB of its keys or values, a wave takes units wave, wave + 4, ..
+  uint32_t rel[L::EACH];
+  bool upper[L::EACH], is_key[L::EACH];
+#pragma unroll
+  for (int i = 0; i < L::EACH; ++i) {
+    int u = wave + WAVES * i;
+    u = u < L::UNITS ? u : L::UNITS - 1;                    // (a wave without a unit of its own repeats the last one)
+    int x = u * 1024 + lane * 16;
+    is_key[i] = x < L::TILE;
+    if (is_key[i]) {
+      const int r = x / L::ROW, place = (x - r * L::ROW) / 16;
+      upper[i] = r >= 16;
+      rel[i] = (r & 15) * L::ROW + (place ^ L::key_turn(r)) * 16;
+    } else {
+      x -= L::TILE;
+      const int half = x / (D * L::VROW);
+      x -= half * D * L::VROW;
+      const int d = x / L::VROW, place = (x - d * L::VROW) / 16;
+      upper[i] = half;
+      rel[i] = d * page * L::ES + (place ^ L::value_turn(d)) * 16;
+    }
+  }
+  const auto* table = (const __attribute__((address_space(4))) int*)(uintptr_t)(tables + (size_t)first_row * max_blocks);
+  const int page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
+  struct Places { int pg[2], off[2]; };
+  auto find = [&](int blk) {
+    Places p;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = blk + 16 * t, pi = page_shift >= 0 ? key >> page_shift : key / page;
+      int pg = table[pi < max_blocks ? pi : max_blocks - 1];
+      pg = pg < 0 ? 0 : pg < pages ? pg : pages - 1;
+      p.pg[t] = pg;
+      p.off[t] = key - pi * page;
+    }
+    return p;
+  };
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds;
+  auto issue = [&](int stage, const Places& p) {
+    const char *k[2], *v[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const size_t head = (size_t)p.pg[t] * Hkv + kvh;
+      k[t] = reinterpret_cast<const char*>(k_cache + (head * page + p.off[t]) * D);
+      v[t] = reinterpret_cast<const char*>(v_cache + head * D * page + p.off[t]);
+    }
+#pragma unroll
+    for (int i = 0; i < L::EACH; ++i) {
+      int u = wave + WAVES * i;
+      u = u < L::UNITS ? u : L::UNITS - 1;
+      const char* base = is_key[i] ? (upper[i] ? k[1] : k[0]) : (upper[i] ? v[1] : v[0]);
+      lane_load_to_lds(base + rel[i], lds0 + stage * 2 * L::TILE + u * 1024);
+    }
+  };
+  const int blk0 = key_begin & ~(BLOCK_KEYS - 1);
+  const int count = key_end > key_begin ? (key_end - blk0 + BLOCK_KEYS - 1) / BLOCK_KEYS : 0;
+#pragma unroll
+  for (int i = 0; i < L::STAGES - 1; ++i)
+    if (i < count) issue(i, find(blk0 + i * BLOCK_KEYS));
+  Places next = find(blk0 + (L::STAGES - 1) * BLOCK_KEYS);     // pages are looked up a block before their loads
+
+  // ---- the wave's columns
+  int limit[CT];                                            // keys that the lane's column sees end here
+  int least = key_end, most = key_begin, tiles = 0;
+  Frag qf[CT][QS];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c0 = col0 + (wave * CT + ct) * 16, c = c0 + col;
+    const bool ok = c < columns;
+    if (c0 < columns) tiles = ct + 1;
+    const int r = first_row + (ok ? c / G : 0), head = kvh * G + (ok ? c % G : 0);
+    const int seen = positions[r] + 1;
+    limit[ct] = ok && seen < key_end ? seen : key_end;
+    least = limit[ct] < least ? limit[ct] : least;
+    if (ok) most = limit[ct] > most ? limit[ct] : most;
+    const T* qp = q + (size_t)r * q_stride + (size_t)head * D;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+      const int d0 = HALF ? s * 32 + kb * 8 : s * 16 + kb * 4;
+      qf[ct][s].q = make_uint4(0, 0, 0, 0);
+      if (ok && d0 < D) {
+        if (q_vec) {
+          qf[ct][s].q = *reinterpret_cast<const uint4*>(qp + d0);
+        } else {
+          T e[16 / sizeof(T)];
+#pragma unroll
+          for (int j = 0; j < (int)(16 / sizeof(T)); ++j) e[j] = load_one(qp + d0 + j);
+          __builtin_memcpy(&qf[ct][s].q, e, 16);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const int a = __shfl_xor(least, o, 64), b = __shfl_xor(most, o, 64);
+    least = a < least ? a : least;
+    most = b > most ? b : most;
+  }
+  least = __builtin_amdgcn_readfirstlane(least);
+  most = __builtin_amdgcn_readfirstlane(most);
+
+  float m[CT], l[CT];
+  f32x4 O[CT][DT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = -INFINITY;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) O[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto key_at = [&](int blk, int j) { return HALF ? blk + 8 * kb + j : blk + 16 * (j >> 2) + 4 * kb + (j & 3); };
+
+  auto compute = [&](const char* stage, int blk) {
+    // ---- scores of 32 keys x 16 CT columns
+    f32x4 S[CT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) S[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int r = HALF ? 8 * (col >> 2) + 4 * t + (col & 3) : 16 * t + col;
+#pragma unroll
+      for (int s = 0; s < QS; ++s) {
+        Frag a;
+        const bool beyond = HALF && D % 32 != 0 && s == KS - 1 && kb >= 2;      // the last step of 32 dims is half empty
+        a.q = *reinterpret_cast<const uint4*>(stage + r * L::ROW + (((beyond ? 0 : 4 * s + kb)) ^ L::key_turn(r)) * 16);
+        if (beyond) a.q = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          if (ct >= tiles) continue;
+          if constexpr (HALF) {
+            S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, qf[ct][s].v, S[ct][t], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w[j]), __uint_as_float(qf[ct][s].w[j]), S[ct][t], 0, 0, 0);
+          }
+        }
+      }
+    }
+    // ---- online softmax, one column a lane's; the maximum follows only when it has grown by more than 2^8, which keeps the sums
+    // as far from overflow as they need be and leaves most blocks without a rescaling
+    const bool partial = blk < key_begin || blk + BLOCK_KEYS > least;
+    float p[CT][8];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if (ct >= tiles) continue;
+      if (partial) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = key_at(blk, j);
+          if (key < key_begin || key >= limit[ct]) S[ct][j >> 2][j & 3] = -INFINITY;
+        }
+      }
+      float mx = S[ct][0][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, S[ct][j >> 2][j & 3]);
+      mx = quad_max(mx) * scale_log2;
+      if (__any(mx > m[ct] + 8.f)) {
+        const float m_new = fmaxf(m[ct], mx);
+        const float alpha = m[ct] == -INFINITY ? 0.f : fast_exp2(m[ct] - m_new);
+        m[ct] = m_new;
+        l[ct] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) O[ct][dt] *= alpha;
+      }
+      const float base = m[ct] == -INFINITY ? 0.f : m[ct];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[ct][j] = fast_exp2(fmaf(S[ct][j >> 2][j & 3], scale_log2, -base));
+        l[ct] += p[ct][j];
+      }
+    }
+    // ---- values
+    const bool stale = blk < key_begin || blk + BLOCK_KEYS > most;      // some keys no column sees: 0 * (whatever is there) must not reach a sum
+    const char* vals = stage + L::TILE;
+    if constexpr (HALF) {
+      Frag pb[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        if (ct >= tiles) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pb[ct].w[j] = pack_bf16(p[ct][2 * j], p[ct][2 * j + 1]);
+      }
+      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      if (stale) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = key_at(blk, 2 * j);
+          keep[j] = (key >= key_begin && key < most ? 0x0000FFFFu : 0u) | (key + 1 >= key_begin && key + 1 < most ? 0xFFFF0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const int d = dt * 16 + col;
+        Frag va;
+        va.q = *reinterpret_cast<const uint4*>(vals + ((kb >> 1) * D + d) * L::VROW + ((kb & 1) ^ L::value_turn(d)) * 16);
+        if (stale) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) va.w[j] &= keep[j];
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          if (ct < tiles) O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pb[ct].v, O[ct][dt], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const int d = dt * 16 + col;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Frag va;
+          va.q = *reinterpret_cast<const uint4*>(vals + (t * D + d) * L::VROW + (kb ^ L::value_turn(d)) * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key_at(blk, 4 * t + i);
+            float a = __uint_as_float(va.w[i]);
+            if (stale && (key < key_begin || key >= most)) a = 0.f;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              if (ct < tiles) O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, p[ct][4 * t + i], O[ct][dt], 0, 0, 0);
+          }
+        }
+      }
+    }
+  };
+
+  for (int n = 0; n < count; ++n) {
+    // block n has landed for every wave, and nobody reads the stage of block n - 1 any more
+    if (n + L::STAGES - 1 <= count) MIE_VMCNT((L::STAGES - 2) * L::EACH);
+    else MIE_VMCNT(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (n + L::STAGES - 1 < count) {
+      issue((n + L::STAGES - 1) % L::STAGES, next);
+      next = find(blk0 + (n + L::STAGES) * BLOCK_KEYS);
+    }
+    if (tiles > 0) compute(lds + (n % L::STAGES) * 2 * L::TILE, blk0 + n * BLOCK_KEYS);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = col0 + (wave * CT + ct) * 16 + col;
+    const float sum = quad_sum(l[ct]);
+    if (c >= columns) continue;
+    const int r = first_row + c / G, head = kvh * G + c % G;
+    const int slot = row_parts[r] + part;
+    if (row_parts[r + 1] - row_parts[r] == 1) {             // nothing to join: the result itself
+      const float sink = head_sinks ? head_sinks[head] * 1.4426950408889634f : sink_log2;
+      const float total = sum + (sink == -INFINITY ? 0.f : m[ct] == -INFINITY ? 1.f : fast_exp2(sink - m[ct]));
+      const float inv = total == 0.f ? 0.f : 1.0f / total;
+      T* o = out + ((size_t)r * Hq + head) * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+      {
+        const f32x4 y = O[ct][dt] * inv;
+        if constexpr (HALF) *reinterpret_cast<uint2*>(o + dt * 16 + 4 * kb) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        else *reinterpret_cast<f32x4*>(o + dt * 16 + 4 * kb) = y;
+      }
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      float* o = o_part + ((size_t)slot * Hq + head) * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        f32x4 y = O[ct][dt] * inv;
+        *reinterpret_cast<f32x4*>(o + dt * 16 + 4 * kb) = y;
+      }
+      if (kb == 0) lse_part[(size_t)slot * Hq + head] = sum == 0.f ? -INFINITY : m[ct] + log2f(sum);
+    }
+  }
+}
+
+// The parts of a row and query head, one wave each: weights from the log-sum-exps, then the parts' outputs, eight asked for together.
+template <typename T>
+__global__ void __launch_bounds__(64)
+join_parts_kernel(const float* __restrict__ o_part, const float* __restrict__ lse_part, T* __restrict__ out,
+                  const int* __restrict__ row_parts, int Hq, float sink_log2, const float* __restrict__ head_sinks) {
+  constexpr int DL = (D + 63) / 64, AHEAD = 8;
+  const int r = blockIdx.x / Hq, head = blockIdx.x - r * Hq, lane = threadIdx.x;
+  const int first = row_parts[r], n = row_parts[r + 1] - first;
+  if (n == 1) return;                                       // written by its only item
+  float M = -INFINITY;
+  for (int j = lane; j < n; j += 64) M = fmaxf(M, lse_part[(size_t)(first + j) * Hq + head]);
+  M = wave_max(M);
+  float acc[DL], W = 0.f;
+#pragma unroll
+  for (int i = 0; i < DL; ++i) acc[i] = 0.f;
+  for (int j0 = 0; j0 < n; j0 += AHEAD) {
+    float w[AHEAD], v[AHEAD][DL];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const size_t at = (size_t)(first + (j0 + j < n ? j0 + j : n - 1)) * Hq + head;
+      w[j] = lse_part[at];
+#pragma unroll
+      for (int i = 0; i < DL; ++i) v[j][i] = o_part[at * D + (lane + 64 * i < D ? lane + 64 * i : 0)];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float x = j0 + j >= n || w[j] == -INFINITY ? 0.f : exp2f(w[j] - M);
+      W += x;
+#pragma unroll
+      for (int i = 0; i < DL; ++i) acc[i] = fmaf(x, v[j][i], acc[i]);
+    }
+  }
+  const float sink = head_sinks ? head_sinks[head] * 1.4426950408889634f : sink_log2;
+  const float total = W + (sink == -INFINITY ? 0.f : M == -INFINITY ? 1.f : exp2f(sink - M));
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+#pragma unroll
+  for (int i = 0; i < DL; ++i)
+    if (lane + 64 * i < D) out[((size_t)r * Hq + head) * D + lane + 64 * i] = from_float<T>(acc[i] * inv);
+}
+
+MIE_EXPORT const char* shared_attention_last_error() { return g_mie_error; }
+MIE_EXPORT int mie_shared_attention_head_dim() { return D; }
+
+template <typename T, int CT>
+static int launch_items(const void* q, long q_stride, const void* k_cache, const void* v_cache, void* out, float* o_part, float* lse_part,
+                        const int* tables, int max_blocks, int pages, const int* positions, const int* items, int num_items,
+                        const int* row_parts, int Hq, int Hkv, int page, float scale, float sink, const float* head_sinks, hipStream_t stream) {
+  auto* kernel = shared_attention_kernel<T, CT>;
+  constexpr int lds = Layout<T>::LDS;
+  if (lds > 65536 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, "shared_prefix_attention")) return -1;
+  const int q_vec = ((uintptr_t)q & 15) == 0 && (q_stride * (long)sizeof(T)) % 16 == 0;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)num_items * Hkv), dim3(WAVES * 64), lds, stream, (const T*)q, q_stride, q_vec,
+                     (const T*)k_cache, (const T*)v_cache, (T*)out, o_part, lse_part, tables, max_blocks, pages, positions,
+                     (const SharedItem*)items, row_parts, Hq, Hkv, page, scale, sink, head_sinks);
+  MIE_CHECK_LAUNCH("shared_prefix_attention");
+  return 0;
+}
+
+// items [num_items, 8], row_parts [rows + 1]: the plan's; o_part [slots, Hq, D] and lse_part [slots, Hq] hold the partial results of rows
+// with several parts (slot row_parts[r] + part).  join: some row has another number of parts than one.  scale, sink: in units of log2 e.
+MIE_EXPORT int mie_shared_attention(const void* q, long q_stride, const void* k_cache, const void* v_cache, void* out, int dtype, float* o_part,
+                                    float* lse_part, const int* tables, int max_blocks, int pages, const int* positions, int rows,
+                                    const int* items, int num_items, int column_tiles, const int* row_parts, int join, int Hq, int Hkv,
+                                    int page, float scale_log2, float sink_log2, const float* head_sinks, hipStream_t stream) {
+  if (rows <= 0) return 0;
+  if (Hkv < 1 || Hq % Hkv || page < 16 || page % 16 || max_blocks < 1 || pages < 1)
+    MIE_FAIL("shared_prefix_attention: %d query heads, %d kv heads, pages of %d keys", Hq, Hkv, page);
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) MIE_FAIL("shared_prefix_attention: caches that do not begin on 16 bytes");
+  if (!(scale_log2 > 0.f)) MIE_FAIL("shared_prefix_attention: the scale must be above 0");
+  if ((long)num_items * Hkv > 0x7FFFFFFFL || (long)rows * Hq > 0x7FFFFFFFL) MIE_FAIL("shared_prefix_attention: too many items or rows");
+  if (num_items > 0) {
+    int rc;
+#define MIE_ITEMS(T, CT) launch_items<T, CT>(q, q_stride, k_cache, v_cache, out, o_part, lse_part, tables, max_blocks, pages, positions, items, \
+                                             num_items, row_parts, Hq, Hkv, page, scale_log2, sink_log2, head_sinks, stream)
+    if (dtype == MIE_BF16) rc = column_tiles == 2 ? MIE_ITEMS(bf16, 2) : MIE_ITEMS(bf16, 1);
+    else rc = column_tiles == 2 ? MIE_ITEMS(float, 2) : MIE_ITEMS(float, 1);
+    if (rc) return rc;
+  }
+  if (join) {
+    if (dtype == MIE_BF16)
+      hipLaunchKernelGGL(join_parts_kernel<bf16>, dim3((unsigned)rows * Hq), dim3(64), 0, stream, o_part, lse_part, (bf16*)out, row_parts, Hq,
+                         sink_log2, head_sinks);
+    else
+      hipLaunchKernelGGL(join_parts_kernel<float>, dim3((unsigned)rows * Hq), dim3(64), 0, stream, o_part, lse_part, (float*)out, row_parts, Hq,
+                         sink_log2, head_sinks);
+    MIE_CHECK_LAUNCH("shared_prefix_attention");
+  }
+  return 0;
+}

@@ -472,6 +472,20 @@ class KernelBackend:
         Returns [T, Hq * D] in act_dtype."""
         raise NotImplementedError
 
+    def plan_shared_prefix(self, groups, contexts, num_q_heads, num_kv_heads, head_dim):
+        """The plan (kernels.shared_prefix.SharedPrefixPlan) of steps of single-token rows whose requests share the first part of
+        their cache: ``groups`` = (rows, keys) of every run of rows, in order, ``keys`` the number of first keys that the rows of the
+        run share (0: none); ``contexts``: for each row the most keys it has while the plan is used (position + 1, or more).  A
+        plan serves every layer of a step, and later steps as long as rows, shared keys and contexts hold."""
+        raise NotImplementedError
+
+    def shared_prefix_attention(self, qkv, num_q_heads, num_kv_heads, head_dim, k_cache, v_cache, group, step, scale, plan, sink=None):
+        """``paged_attention`` (no window) of a step of single-token rows under ``plan``: the shared keys of a run are read through
+        the block table of the run's first row and once for all its rows, the others through each row's own table.  A row at position p
+        sees keys 0 .. p; one at a position below 0 sees none and gives zeros.  ``scale`` > 0; ``sink`` as in ``paged_attention``.
+        Returns [T, Hq * D] in act_dtype."""
+        raise NotImplementedError
+
     def sample(self, logits, temperatures, seeds, counters, out=None, rules=None):
         """Per row: argmax(logits) if temperature == 0, else argmax(logits / temperature + g)
         with Gumbel noise g from (seed, counter, vocabulary index).  -> [R] int32 (``out`` if given).  The lowest index among

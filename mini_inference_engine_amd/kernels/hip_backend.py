@@ -18,6 +18,7 @@ import torch
 
 from . import library
 from .api import KernelBackend, Normed, Sink
+from .shared_prefix import SharedPrefixPlan
 
 F32, BF16 = 0, 1
 
@@ -1971,6 +1972,59 @@ class HipBackend(KernelBackend):
                                                               step.num_rows, longest, Hq, Hkv, D, page, float(scale), window,
                                                               int(getattr(step, "max_context", 0) or 0), self._stream()))
         return True
+
+    # ---- rows that share the first part of their cache (csrc/shared_attention.hip)
+    def plan_shared_prefix(self, groups, contexts, num_q_heads, num_kv_heads, head_dim):
+        return SharedPrefixPlan(groups, contexts, num_q_heads, num_kv_heads, head_dim, self.device,
+                                torch.cuda.get_device_properties(self._device_index).multi_processor_count)
+
+    def shared_prefix_attention(self, qkv, num_q_heads, num_kv_heads, head_dim, k_cache, v_cache, group, step, scale, plan, sink=None):
+        Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim
+        T, page, bt = self._check_shared(qkv, Hq, Hkv, D, k_cache, v_cache, group, step, scale, plan)
+        head_sinks, sink_log2 = None, float("-inf")
+        if isinstance(sink, torch.Tensor):
+            self._on_device(sink)
+            self._f32_vector(sink, Hq, "shared_prefix_attention: sinks")
+            head_sinks = sink
+        elif sink is not None:
+            sink_log2 = float(sink) * self.LOG2_E
+        self._on_device(qkv, k_cache, v_cache, bt, step.positions, plan.items)
+        lib = self.lib("shared_attention", (f"-DHEAD_DIM={D}",))
+        out = torch.empty((T, Hq * D), dtype=qkv.dtype, device=qkv.device)
+        parts = None
+        if plan.join:               # partial outputs, then their log-sum-exps
+            parts = torch.empty(plan.num_parts * Hq * (D + 1), dtype=torch.float32, device=qkv.device)
+        at = None if parts is None else parts.data_ptr()
+        library.check(lib, lib.mie_shared_attention(
+            qkv.data_ptr(), qkv.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _code(qkv.dtype), at,
+            None if at is None else at + 4 * plan.num_parts * Hq * D, bt.data_ptr(), bt.shape[1], k_cache.shape[0], step.positions.data_ptr(), T,
+            plan.items.data_ptr(), plan.num_items, plan.column_tiles, plan.row_parts.data_ptr(), int(plan.join), Hq, Hkv, page,
+            float(scale) * self.LOG2_E, sink_log2, _ptr(head_sinks), self._stream()))
+        return out
+
+    LOG2_E = 1.4426950408889634
+
+    def _check_shared(self, qkv, Hq, Hkv, D, k_cache, v_cache, group, step, scale, plan):
+        T, page, bt = self._check_attention(qkv, Hq, Hkv, D, k_cache, v_cache, group, step)
+        if D % 16 or not 16 <= D <= 256 or page % 16:
+            raise ValueError(f"shared_prefix_attention: heads of {D} numbers, pages of {page} keys (multiples of 16, heads up to 256)")
+        if qkv.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"shared_prefix_attention: float32 or bfloat16, not {qkv.dtype}")
+        if step.num_decode_rows != T or step.num_rows != T:
+            raise ValueError("shared_prefix_attention: a step of single-token rows only")
+        if not isinstance(plan, SharedPrefixPlan) or (plan.num_rows, plan.num_q_heads, plan.num_kv_heads, plan.head_dim) != (T, Hq, Hkv, D):
+            raise ValueError(f"shared_prefix_attention: the plan is not one of {T} rows, {Hq} / {Hkv} heads of {D}")
+        if plan.max_context > bt.shape[1] * page or step.max_context > plan.max_context:
+            raise ValueError(f"shared_prefix_attention: a plan for contexts up to {plan.max_context}; the step's reach {step.max_context}, "
+                             f"its block tables {bt.shape[1]} pages of {page}")
+        ends = step.host.get("row_context") if step.host else None
+        if ends is not None and (ends > plan.contexts).any():
+            raise ValueError("shared_prefix_attention: a row's context is beyond the one it was planned for")
+        if not 0 < scale < float("inf"):
+            raise ValueError(f"shared_prefix_attention: scale {scale}")
+        if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+            raise ValueError("shared_prefix_attention: caches must begin on 16 bytes")
+        return T, page, bt
 
     def _check_logits(self, what, logits):
         if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:

@@ -171,6 +171,10 @@ register_kernel_module("prefill_attention_bf16", {
     "mie_step_attention": [P, L, P, P, P, P, P, P, I, P, I, I, I, P, P, P, I, I, I, I, I, I, F, I, F, P],
     "mie_prefill_attention_kept": [P, L, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, F, I, I, P, P],
 }, variants=_head_variants, flags=["-mllvm", "-amdgpu-mfma-vgpr-form"])
+register_kernel_module("shared_attention", {
+    "mie_shared_attention_head_dim": [],
+    "mie_shared_attention": [P, L, P, P, P, I, P, P, P, I, I, P, I, P, I, I, P, I, I, I, I, F, F, P, P],
+}, variants=_head_variants, flags=["-mllvm", "-amdgpu-mfma-vgpr-form"])
 # lt_gemm: host code only, the engine's own way into the library's matrix products (hipBLASLt) with the choice of
 # kernel per shape kept here.
 register_kernel_module("lt_gemm", {
