@@ -16,6 +16,9 @@
 #pragma clang fp contract(off)      // the formulas' roundings, one by one
 
 constexpr int RULE_THREADS = 256;
+constexpr int RULE_SLICE = 4096;                       // most tokens of the vocabulary that a workgroup takes
+constexpr int RULE_AHEAD = RULE_SLICE / (RULE_THREADS * 4);
+typedef int int4_any __attribute__((ext_vector_type(4), aligned(4)));      // four numbers wherever they begin
 constexpr uint32_t SEEN = 0x80000000u, BIASED = 0x40000000u, TIMES = 0x3FFFFFFFu;
 
 struct Rules {
@@ -99,20 +102,52 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
     const int m = rules.mask_row[r];
     if (m >= 0 && m < rules.num_masks) mask = rules.masks + (size_t)m * rules.mask_ld;
   }
+  // the slice's logits and mask are asked for before the text is read
+  const float* z0 = logits + (size_t)r * ld + begin;
+  const int n4 = VEC ? n & ~3 : 0;
+  float4 z[RULE_AHEAD];
+  uint32_t bits[RULE_AHEAD];
+#pragma unroll
+  for (int k = 0; k < RULE_AHEAD; ++k) {
+    const int i = (k * RULE_THREADS + tid) * 4;
+    if (i < n4) {
+      z[k] = *reinterpret_cast<const float4*>(z0 + i);
+      bits[k] = mask ? mask[(begin + i) >> 5] >> ((begin + i) & 31) : 15u;
+    }
+  }
   const bool counted = length > 0 || listed > 0;                      // (the same in the whole workgroup)
   if (counted) {
-    for (int i = tid; i < n; i += RULE_THREADS) {
-      words[i] = 0;
-      if (listed > 0) bias_at[i] = 0;
+    const int zeros = (n + 3) / 4;
+    for (int i = tid; i < zeros; i += RULE_THREADS) {
+      reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+      if (listed > 0) reinterpret_cast<uint4*>(bias_at)[i] = make_uint4(0, 0, 0, 0);
     }
     __syncthreads();
-    for (int i = tid; i < length; i += RULE_THREADS) {
-      const unsigned at = (unsigned)(text[i] - begin);                // what is no token of the vocabulary is in no slice
+    auto count = [&](int token, int i) {
+      const unsigned at = (unsigned)(token - begin);                  // what is no token of the vocabulary is in no slice
       if (at < (unsigned)n) {
         atomicOr(&words[at], SEEN);
         if (i >= prompt) atomicAdd(&words[at], 1u);
       }
+    };
+    const int length4 = length & ~3;
+    constexpr int READS = 4;                                          // on their way together
+    for (int i0 = tid * 4; i0 < length4; i0 += READS * RULE_THREADS * 4) {
+      int4_any t[READS];
+#pragma unroll
+      for (int k = 0; k < READS; ++k) {
+        const int i = i0 + k * RULE_THREADS * 4;
+        t[k] = *reinterpret_cast<const int4_any*>(text + (i < length4 ? i : i0));
+      }
+#pragma unroll
+      for (int k = 0; k < READS; ++k) {
+        const int i = i0 + k * RULE_THREADS * 4;
+        if (i >= length4) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) count(t[k][j], i + j);
+      }
     }
+    if (length4 + tid < length) count(text[length4 + tid], length4 + tid);
     for (int i = tid; i < listed; i += RULE_THREADS) {
       const unsigned at = (unsigned)(list[i] - begin);
       if (at < (unsigned)n) {
@@ -123,7 +158,6 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
     __syncthreads();
   }
 
-  const float* z0 = logits + (size_t)r * ld + begin;
   float* o0 = CHOOSE ? nullptr : out + (size_t)r * out_ld + begin;
   bool noisy = false;
   float inv_t = 1.f;
@@ -138,17 +172,17 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   }
   float bv = -INFINITY;
   int bi = 0x7FFFFFFF;
-  const int n4 = VEC ? n & ~3 : 0;
-  for (int i = tid * 4; i < n4; i += RULE_THREADS * 4) {
-    const float4 z = *reinterpret_cast<const float4*>(z0 + i);
+#pragma unroll
+  for (int k = 0; k < RULE_AHEAD; ++k) {
+    const int i = (k * RULE_THREADS + tid) * 4;
+    if (i >= n4) break;
     uint4 w = make_uint4(0, 0, 0, 0);
     if (counted) w = *reinterpret_cast<const uint4*>(words + i);
-    const uint32_t bits = mask ? mask[(begin + i) >> 5] >> ((begin + i) & 31) : 15u;
     float4 y;
-    y.x = bits & 1 ? apply_rules(z.x, w.x, i, row) : -INFINITY;
-    y.y = bits & 2 ? apply_rules(z.y, w.y, i + 1, row) : -INFINITY;
-    y.z = bits & 4 ? apply_rules(z.z, w.z, i + 2, row) : -INFINITY;
-    y.w = bits & 8 ? apply_rules(z.w, w.w, i + 3, row) : -INFINITY;
+    y.x = bits[k] & 1 ? apply_rules(z[k].x, w.x, i, row) : -INFINITY;
+    y.y = bits[k] & 2 ? apply_rules(z[k].y, w.y, i + 1, row) : -INFINITY;
+    y.z = bits[k] & 4 ? apply_rules(z[k].z, w.z, i + 2, row) : -INFINITY;
+    y.w = bits[k] & 8 ? apply_rules(z[k].w, w.w, i + 3, row) : -INFINITY;
     if (CHOOSE) {
       sample_consider(y.x, begin + i, noisy, inv_t, key, bv, bi);
       sample_consider(y.y, begin + i + 1, noisy, inv_t, key, bv, bi);
@@ -220,7 +254,7 @@ MIE_EXPORT const char* logit_rules_last_error() { return g_mie_error; }
 // Tokens of the vocabulary that a workgroup takes.
 MIE_EXPORT int mie_rules_slice(int rows, int V) {
   int slice = 1024;
-  while (slice < 4096 && (long)rows * ((V + slice - 1) / slice) > 4L * mie_compute_units()) slice *= 2;
+  while (slice < RULE_SLICE && (long)rows * ((V + slice - 1) / slice) > 4L * mie_compute_units()) slice *= 2;
   return slice;
 }
 
