@@ -15,10 +15,14 @@
 #include "sampling.hpp"
 #pragma clang fp contract(off)      // the formulas' roundings, one by one
 
-constexpr int RULE_THREADS = 256;
-constexpr int RULE_SLICE = 4096;                       // most tokens of the vocabulary that a workgroup takes
-constexpr int RULE_AHEAD = RULE_SLICE / (RULE_THREADS * 4);
-typedef int int4_any __attribute__((ext_vector_type(4), aligned(4)));      // four numbers wherever they begin
+// Two ways of dividing a row: slices of 4,096 tokens on workgroups of 256 threads, joined by a second launch, and the
+// whole row on a workgroup of 1,024 threads that goes through slices of 32,768.
+constexpr int PART_THREADS = 256, ROW_THREADS = 1024;
+constexpr int ahead_of(int threads) { return threads == ROW_THREADS ? 8 : 4; }        // reads of four logits a thread and slice, all on their way at once
+constexpr int slice_of(int threads) { return threads * 4 * ahead_of(threads); }
+// four numbers wherever they begin
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 constexpr uint32_t SEEN = 0x80000000u, BIASED = 0x40000000u, TIMES = 0x3FFFFFFFu;
 
 struct Rules {
@@ -45,11 +49,10 @@ __device__ __forceinline__ int clamp_int(int x, int low, int high) { return x < 
 
 struct RowRules {
   float repetition, presence, frequency;
-  const float* bias_values;      // of the row's list
-  const int* bias_at;            // LDS: 1 + the place in that list, of tokens whose word has BIASED
 };
 
-__device__ __forceinline__ float apply_rules(float z, uint32_t w, int i, const RowRules& r) {
+// penalties
+__device__ __forceinline__ float apply_rules(float z, uint32_t w, const RowRules& r) {
   if (w == 0) return z;
   if (w & SEEN) z = z > 0.f ? z / r.repetition : z * r.repetition;
   const uint32_t c = w & TIMES;
@@ -57,25 +60,23 @@ __device__ __forceinline__ float apply_rules(float z, uint32_t w, int i, const R
     z = z - r.frequency * (float)c;
     z = z - r.presence;
   }
-  if (w & BIASED) z = z + r.bias_values[r.bias_at[i] - 1];
   return z;
 }
 
-// Grid (slices, rows).  CHOOSE: the slice's best candidate to best_v, best_i [rows, slices], or, of a row that is one slice, the
-// token to ``chosen``; else the adjusted logits to ``out``.  VEC: rows of logits (and of ``out``) begin on 16 bytes.
-template <bool CHOOSE, bool VEC>
-__global__ void __launch_bounds__(RULE_THREADS)
+// Grid (workgroups a row, rows); a workgroup takes every gridDim.x-th slice.  CHOOSE: its best candidate to best_v, best_i [rows,
+// workgroups], or, of a row that has one workgroup, the token to ``chosen``; else the adjusted logits to ``out``.
+template <bool CHOOSE, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float* out, long out_ld,
              const float* __restrict__ temperatures, const long long* __restrict__ seeds, const int* __restrict__ counters,
              float* __restrict__ best_v, int* __restrict__ best_i, int* __restrict__ chosen) {
-  extern __shared__ __align__(16) uint32_t words[];                   // [slice], then, with biases, [slice] places in the list
-  int* bias_at = reinterpret_cast<int*>(words + slice);
-  __shared__ float wave_v[RULE_THREADS / 64];
-  __shared__ int wave_i[RULE_THREADS / 64];
-  const int r = blockIdx.y, begin = blockIdx.x * slice, n = min(slice, V - begin);
-  const int tid = threadIdx.x;
+  constexpr int AHEAD = ahead_of(THREADS);
+  extern __shared__ __align__(16) uint32_t words[];                   // [slice]
+  __shared__ float wave_v[THREADS / 64];
+  __shared__ int wave_i[THREADS / 64];
+  const int r = blockIdx.y, tid = threadIdx.x;
 
-  RowRules row{1.f, 0.f, 0.f, nullptr, bias_at};
+  RowRules row{1.f, 0.f, 0.f};
   int length = 0, prompt = 0;
   const int* text = nullptr;
   if (rules.history) {
@@ -91,74 +92,18 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   }
   int listed = 0;
   const int* list = nullptr;
+  const float* list_values = nullptr;
   if (rules.bias_starts) {
     const int a = clamp_int(rules.bias_starts[r], 0, rules.biases), b = clamp_int(rules.bias_starts[r + 1], a, rules.biases);
     listed = b - a;
     list = rules.bias_tokens + a;
-    row.bias_values = rules.bias_values + a;
+    list_values = rules.bias_values + a;
   }
   const uint32_t* mask = nullptr;
   if (rules.masks) {
     const int m = rules.mask_row[r];
     if (m >= 0 && m < rules.num_masks) mask = rules.masks + (size_t)m * rules.mask_ld;
   }
-  // the slice's logits and mask are asked for before the text is read
-  const float* z0 = logits + (size_t)r * ld + begin;
-  const int n4 = VEC ? n & ~3 : 0;
-  float4 z[RULE_AHEAD];
-  uint32_t bits[RULE_AHEAD];
-#pragma unroll
-  for (int k = 0; k < RULE_AHEAD; ++k) {
-    const int i = (k * RULE_THREADS + tid) * 4;
-    if (i < n4) {
-      z[k] = *reinterpret_cast<const float4*>(z0 + i);
-      bits[k] = mask ? mask[(begin + i) >> 5] >> ((begin + i) & 31) : 15u;
-    }
-  }
-  const bool counted = length > 0 || listed > 0;                      // (the same in the whole workgroup)
-  if (counted) {
-    const int zeros = (n + 3) / 4;
-    for (int i = tid; i < zeros; i += RULE_THREADS) {
-      reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
-      if (listed > 0) reinterpret_cast<uint4*>(bias_at)[i] = make_uint4(0, 0, 0, 0);
-    }
-    __syncthreads();
-    auto count = [&](int token, int i) {
-      const unsigned at = (unsigned)(token - begin);                  // what is no token of the vocabulary is in no slice
-      if (at < (unsigned)n) {
-        atomicOr(&words[at], SEEN);
-        if (i >= prompt) atomicAdd(&words[at], 1u);
-      }
-    };
-    const int length4 = length & ~3;
-    constexpr int READS = 4;                                          // on their way together
-    for (int i0 = tid * 4; i0 < length4; i0 += READS * RULE_THREADS * 4) {
-      int4_any t[READS];
-#pragma unroll
-      for (int k = 0; k < READS; ++k) {
-        const int i = i0 + k * RULE_THREADS * 4;
-        t[k] = *reinterpret_cast<const int4_any*>(text + (i < length4 ? i : i0));
-      }
-#pragma unroll
-      for (int k = 0; k < READS; ++k) {
-        const int i = i0 + k * RULE_THREADS * 4;
-        if (i >= length4) break;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) count(t[k][j], i + j);
-      }
-    }
-    if (length4 + tid < length) count(text[length4 + tid], length4 + tid);
-    for (int i = tid; i < listed; i += RULE_THREADS) {
-      const unsigned at = (unsigned)(list[i] - begin);
-      if (at < (unsigned)n) {
-        atomicOr(&words[at], BIASED);
-        atomicMax(&bias_at[at], i + 1);
-      }
-    }
-    __syncthreads();
-  }
-
-  float* o0 = CHOOSE ? nullptr : out + (size_t)r * out_ld + begin;
   bool noisy = false;
   float inv_t = 1.f;
   uint32_t key = 0;
@@ -172,32 +117,106 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   }
   float bv = -INFINITY;
   int bi = 0x7FFFFFFF;
+  const bool counted = length > 0 || listed > 0;                      // (the same in the whole workgroup)
+  for (int begin = blockIdx.x * slice; begin < V; begin += gridDim.x * slice) {
+    const int n = min(slice, V - begin), n4 = n & ~3;
+    const float* z0 = logits + (size_t)r * ld + begin;
+    // the slice's logits and mask are asked for before the text is read
+    f32x4_any z[AHEAD];
+    uint32_t bits[AHEAD];
 #pragma unroll
-  for (int k = 0; k < RULE_AHEAD; ++k) {
-    const int i = (k * RULE_THREADS + tid) * 4;
-    if (i >= n4) break;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (counted) w = *reinterpret_cast<const uint4*>(words + i);
-    float4 y;
-    y.x = bits[k] & 1 ? apply_rules(z[k].x, w.x, i, row) : -INFINITY;
-    y.y = bits[k] & 2 ? apply_rules(z[k].y, w.y, i + 1, row) : -INFINITY;
-    y.z = bits[k] & 4 ? apply_rules(z[k].z, w.z, i + 2, row) : -INFINITY;
-    y.w = bits[k] & 8 ? apply_rules(z[k].w, w.w, i + 3, row) : -INFINITY;
-    if (CHOOSE) {
-      sample_consider(y.x, begin + i, noisy, inv_t, key, bv, bi);
-      sample_consider(y.y, begin + i + 1, noisy, inv_t, key, bv, bi);
-      sample_consider(y.z, begin + i + 2, noisy, inv_t, key, bv, bi);
-      sample_consider(y.w, begin + i + 3, noisy, inv_t, key, bv, bi);
-    } else {
-      *reinterpret_cast<float4*>(o0 + i) = y;
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = (k * THREADS + tid) * 4;
+      if (i < n4) {
+        z[k] = *reinterpret_cast<const f32x4_any*>(z0 + i);
+        bits[k] = mask ? mask[(begin + i) >> 5] >> ((begin + i) & 31) : 15u;
+      }
     }
-  }
-  for (int i = n4 + tid; i < n; i += RULE_THREADS) {
-    const bool may = !mask || (mask[(begin + i) >> 5] >> ((begin + i) & 31) & 1);
-    const float z = z0[i];
-    const float y = may ? apply_rules(z, counted ? words[i] : 0, i, row) : -INFINITY;
-    if (CHOOSE) sample_consider(y, begin + i, noisy, inv_t, key, bv, bi);
-    else o0[i] = y;
+    if (counted) {
+      if (begin != (int)blockIdx.x * slice) __syncthreads();          // the words of the slice before have been read
+      const int zeros = (n + 3) / 4;
+      for (int i = tid; i < zeros; i += THREADS) {
+        reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+      }
+      __syncthreads();
+      auto count = [&](int token, int i) {
+        const unsigned at = (unsigned)token - (unsigned)begin;        // what is no token of the vocabulary is in no slice
+        if (at < (unsigned)n) {
+          atomicOr(&words[at], SEEN);
+          if (i >= prompt) atomicAdd(&words[at], 1u);
+        }
+      };
+      const int length4 = length & ~3;
+      constexpr int READS = 4;                                        // on their way together
+      for (int i0 = tid * 4; i0 < length4; i0 += READS * THREADS * 4) {
+        i32x4_any t[READS];
+#pragma unroll
+        for (int k = 0; k < READS; ++k) {
+          const int i = i0 + k * THREADS * 4;
+          t[k] = *reinterpret_cast<const i32x4_any*>(text + (i < length4 ? i : i0));
+        }
+#pragma unroll
+        for (int k = 0; k < READS; ++k) {
+          const int i = i0 + k * THREADS * 4;
+          if (i >= length4) break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) count(t[k][j], i + j);
+        }
+      }
+      if (length4 + tid < length) count(text[length4 + tid], length4 + tid);
+      for (int i = tid; i < listed; i += THREADS) {
+        const unsigned at = (unsigned)list[i] - (unsigned)begin;
+        if (at < (unsigned)n) atomicOr(&words[at], BIASED);
+      }
+      __syncthreads();
+    }
+    float* o0 = CHOOSE ? nullptr : out + (size_t)r * out_ld + begin;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = (k * THREADS + tid) * 4;
+      if (i >= n4) break;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (counted) w = *reinterpret_cast<const uint4*>(words + i);
+      f32x4_any y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t wj = j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
+        y[j] = bits[k] >> j & 1 ? apply_rules(z[k][j], wj, row) : -INFINITY;
+        if (wj & BIASED) y[j] = z[k][j];                              // left to the list, below
+        else if (CHOOSE) sample_consider(y[j], begin + i + j, noisy, inv_t, key, bv, bi);
+      }
+      if (!CHOOSE) *reinterpret_cast<f32x4_any*>(o0 + i) = y;
+    }
+    if (n4 + tid < n) {                                               // up to three at the end of the row
+      const int i = n4 + tid;
+      const uint32_t w = counted ? words[i] : 0;
+      const bool may = !mask || (mask[(begin + i) >> 5] >> ((begin + i) & 31) & 1);
+      const float z1 = z0[i], y = w & BIASED ? z1 : may ? apply_rules(z1, w, row) : -INFINITY;
+      if (!CHOOSE) o0[i] = y;
+      else if (!(w & BIASED)) sample_consider(y, begin + i, noisy, inv_t, key, bv, bi);
+    }
+    // The tokens with a bias, a thread an entry of the list, the list's end first.  Of several entries of a token the last one
+    // has it: within a round the largest thread that asks for it, and what a round has settled has lost its mark for those before.
+    for (int i0 = (listed - 1) / THREADS * THREADS; listed > 0 && i0 >= 0; i0 -= THREADS) {
+      const int e = i0 + tid;
+      const unsigned at = e < listed ? (unsigned)list[e] - (unsigned)begin : ~0u;
+      const bool mine = at < (unsigned)n;
+      __syncthreads();                                                // (and the logits as they were are in memory)
+      const uint32_t w = mine ? words[at] : 0;
+      const bool asks = w & BIASED;
+      __syncthreads();
+      if (asks) words[at] = 0;
+      __syncthreads();
+      if (asks) atomicMax(&words[at], (uint32_t)tid + 1);
+      __syncthreads();
+      if (asks && words[at] == (uint32_t)tid + 1) {
+        const int v = begin + (int)at;
+        const bool may = !mask || (mask[v >> 5] >> (v & 31) & 1);
+        const float y = may ? apply_rules(z0[at], w & ~BIASED, row) + list_values[e] : -INFINITY;
+        if (CHOOSE) sample_consider(y, v, noisy, inv_t, key, bv, bi);
+        else o0[at] = y;
+      }
+    }
   }
   if (!CHOOSE) return;
 #pragma unroll
@@ -209,7 +228,7 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   if ((tid & 63) == 0) { wave_v[tid >> 6] = bv; wave_i[tid >> 6] = bi; }
   __syncthreads();
   if (tid == 0) {
-    for (int i = 1; i < RULE_THREADS / 64; ++i) sample_better(wave_v[i], wave_i[i], bv, bi);
+    for (int i = 1; i < THREADS / 64; ++i) sample_better(wave_v[i], wave_i[i], bv, bi);
     if (gridDim.x == 1) {
       chosen[r] = bi == 0x7FFFFFFF ? 0 : bi;
     } else {
@@ -251,15 +270,17 @@ record_tokens_kernel(int* __restrict__ history, long ld, int slots, int most, co
 
 MIE_EXPORT const char* logit_rules_last_error() { return g_mie_error; }
 
-// Tokens of the vocabulary that a workgroup takes.
-MIE_EXPORT int mie_rules_slice(int rows, int V) {
-  int slice = 1024;
-  while (slice < RULE_SLICE && (long)rows * ((V + slice - 1) / slice) > 4L * mie_compute_units()) slice *= 2;
-  return slice;
+// Workgroups a row: one, or one for each slice.
+MIE_EXPORT int mie_rules_slices(int rows, int V) {
+  const int slices = (V + slice_of(PART_THREADS) - 1) / slice_of(PART_THREADS);
+#ifdef XROW
+  return rows >= XROW ? 1 : slices;
+#endif
+  return slices;
 }
 
 static int check_rules(const char* what, const Rules& r, int rows, int V, long ld) {
-  if (V <= 0 || ld < V) MIE_FAIL("%s: vocabulary %d, leading dim %ld", what, V, ld);
+  if (V <= 0 || V > 1 << 30 || ld < V) MIE_FAIL("%s: vocabulary %d, leading dim %ld", what, V, ld);
   if (rows > 65535) MIE_FAIL("%s: %d rows, at most 65535", what, rows);
   if (r.history && (r.most < 0 || r.history_ld < r.most || r.slots < 0)) MIE_FAIL("%s: history of %d slots, %d positions, %ld apart", what, r.slots, r.most, r.history_ld);
   if (r.masks && (r.mask_ld < (V + 31) / 32 || r.num_masks < 0)) MIE_FAIL("%s: masks of %ld words for a vocabulary of %d", what, r.mask_ld, V);
@@ -272,11 +293,13 @@ static int launch_rules(const char* what, const float* logits, long ld, const Ru
                         hipStream_t stream) {
   if (rows <= 0) return 0;
   if (check_rules(what, rules, rows, V, ld)) return -1;
-  const int slice = mie_rules_slice(rows, V), slices = (V + slice - 1) / slice;
-  const int lds = slice * 4 * (rules.bias_starts ? 2 : 1);
-  const bool vec = ((uintptr_t)logits & 15) == 0 && (ld & 3) == 0 && (CHOOSE || (((uintptr_t)out & 15) == 0 && (out_ld & 3) == 0));
-  auto* kernel = vec ? rules_kernel<CHOOSE, true> : rules_kernel<CHOOSE, false>;
-  hipLaunchKernelGGL(kernel, dim3(slices, rows), dim3(RULE_THREADS), lds, stream, logits, ld, rules, V, slice, out, out_ld, temperatures,
+  const int slices = mie_rules_slices(rows, V);
+  const int threads = slices > 1 ? PART_THREADS : ROW_THREADS;
+  const int slice = V < slice_of(threads) ? (V + 3) & ~3 : slice_of(threads);
+  const int lds = slice * 4;
+  auto* kernel = slices > 1 ? rules_kernel<CHOOSE, PART_THREADS> : rules_kernel<CHOOSE, ROW_THREADS>;
+  if (lds > 65536 - 256 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, what)) return -1;
+  hipLaunchKernelGGL(kernel, dim3(slices, rows), dim3(threads), lds, stream, logits, ld, rules, V, slice, out, out_ld, temperatures,
                      seeds, counters, best_v, best_i, chosen);
   MIE_CHECK_LAUNCH(what);
   if (CHOOSE && slices > 1) {
@@ -299,7 +322,7 @@ MIE_EXPORT int mie_adjust_logits(const float* logits, long ld, RULE_ARGS, float*
   return launch_rules<false>("adjust_logits", logits, ld, RULES, rows, V, out, out_ld, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, stream);
 }
 
-// best_v, best_i: [rows, slices of mie_rules_slice] (unused where that is one)
+// best_v, best_i: [rows, mie_rules_slices] (unused where that is one)
 MIE_EXPORT int mie_choose_by_rules(const float* logits, long ld, RULE_ARGS, const float* temperatures, const long long* seeds,
                                    const int* counters, float* best_v, int* best_i, int* chosen, int rows, int V, hipStream_t stream) {
   return launch_rules<true>("sample", logits, ld, RULES, rows, V, nullptr, 0, temperatures, seeds, counters, best_v, best_i, chosen, stream);

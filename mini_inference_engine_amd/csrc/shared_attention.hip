@@ -14,8 +14,11 @@
 // one of the second product's steps of 4 keys takes one number of each lane group.  Probabilities never leave registers.
 #include "attention_bf16_common.hpp"
 #include "launch.hpp"
+#include <type_traits>
 
 constexpr int WAVES = 4;
+// Tiles of 16 columns a wave: two, as far as their outputs have room in the registers.
+constexpr int mie_shared_most_tiles() { return D <= 128 ? 2 : 1; }
 
 // 16 bytes a lane from a lane's own address into the LDS at byte `at` + 16 lane (waits are the kernel's own)
 __device__ __forceinline__ void lane_load_to_lds(const char* from, uint32_t at) {
@@ -38,15 +41,18 @@ struct SharedItem {
   int unused0, unused1;
 };
 
-template <typename T> struct Kind;
-template <> struct Kind<bf16> {
-  static constexpr int STAGES = D <= 32 ? 6 : D <= 64 ? 4 : 3;
-};
-template <> struct Kind<float> {
-  static constexpr int STAGES = D <= 64 ? 4 : D <= 128 ? 3 : 2;
-};
+#ifndef XST1
+#define XST1 3
+#endif
+#ifndef XST2
+#define XST2 5
+#endif
+template <typename T, int CT> constexpr int stages_of() {
+  if (sizeof(T) == 2) return D <= 32 ? 8 : D <= 64 ? 6 : D <= 128 ? (CT == 2 ? XST2 : XST1) : 3;
+  return D <= 64 ? 4 : D <= 128 ? 3 : 2;
+}
 
-template <typename T>
+template <typename T, int CT>
 struct Layout {
   static constexpr int ES = sizeof(T);
   static constexpr int ROW = D * ES;                        // bytes of a key
@@ -56,7 +62,7 @@ struct Layout {
   static constexpr int TILE = 32 * ROW;                     // keys of a block; values take as much
   static constexpr int UNITS = 2 * TILE / 1024;             // of a block's loads
   static constexpr int EACH = (UNITS + WAVES - 1) / WAVES;  // a wave's
-  static constexpr int STAGES = Kind<T>::STAGES;
+  static constexpr int STAGES = stages_of<T, CT>();
   static constexpr int LDS = STAGES * 2 * TILE;
   // 16-byte places are turned by what tells the rows apart that are read at once, so that they lie in different banks
   static __device__ __forceinline__ int key_turn(int r) { return (ES == 2 ? (r & 3) | ((r >> 3 & 1) << 2) : r & 7) & TURN; }
@@ -67,13 +73,13 @@ __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ bf16 load_one(const bf16* p) { return *p; }
 
 template <typename T, int CT>
-__global__ void __launch_bounds__(WAVES * 64)
+__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 2 && D <= 128 ? 2 : 1)
 shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
                         T* __restrict__ out, float* __restrict__ o_part, float* __restrict__ lse_part, const int* __restrict__ tables,
                         int max_blocks, int pages, const int* __restrict__ positions, const SharedItem* __restrict__ items,
                         const int* __restrict__ row_parts, int Hq, int Hkv, int page, float scale_log2, float sink_log2,
                         const float* __restrict__ head_sinks) {
-  using L = Layout<T>;
+  using L = Layout<T, CT>;
   constexpr bool HALF = sizeof(T) == 2;
   constexpr int QS = HALF ? KS : D / 16;                    // 16-byte pieces of a column's query that a lane holds
   extern __shared__ __align__(1024) char lds[];
@@ -112,17 +118,33 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     }
   }
   const auto* table = (const __attribute__((address_space(4))) int*)(uintptr_t)(tables + (size_t)first_row * max_blocks);
-  const int page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
+  // Where a block's keys lie: its halves of 16 keys are in one page each.  Followed from block to block by additions.
+  const int blk0 = key_begin & ~(BLOCK_KEYS - 1);
+  const uint64_t page_bytes = (uint64_t)(uint32_t)Hkv * page * L::ROW;       // of keys; of values as well
+  const char* const keys0 = reinterpret_cast<const char*>(k_cache) + (size_t)kvh * page * L::ROW;
+  const char* const vals0 = reinterpret_cast<const char*>(v_cache) + (size_t)kvh * page * L::ROW;
+  int index[2], off[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    index[t] = (blk0 + 16 * t) / page;
+    off[t] = blk0 + 16 * t - index[t] * page;
+  }
   struct Places { int pg[2], off[2]; };
-  auto find = [&](int blk) {
+  auto find = [&]() {                                       // of the next block in order
     Places p;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int key = blk + 16 * t, pi = page_shift >= 0 ? key >> page_shift : key / page;
-      int pg = table[pi < max_blocks ? pi : max_blocks - 1];
-      pg = pg < 0 ? 0 : pg < pages ? pg : pages - 1;
-      p.pg[t] = pg;
-      p.off[t] = key - pi * page;
+      p.pg[t] = table[index[t] < max_blocks ? index[t] : max_blocks - 1];
+      p.off[t] = off[t];
+      if (page == 16) {
+        index[t] += 2;
+      } else {
+        off[t] += BLOCK_KEYS;
+        if (off[t] >= page) {
+          off[t] -= page;
+          ++index[t];
+        }
+      }
     }
     return p;
   };
@@ -131,9 +153,10 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     const char *k[2], *v[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const size_t head = (size_t)p.pg[t] * Hkv + kvh;
-      k[t] = reinterpret_cast<const char*>(k_cache + (head * page + p.off[t]) * D);
-      v[t] = reinterpret_cast<const char*>(v_cache + head * D * page + p.off[t]);
+      const uint32_t pg = (uint32_t)p.pg[t] < (uint32_t)pages ? p.pg[t] : 0;
+      const uint64_t at = pg * page_bytes;
+      k[t] = keys0 + at + p.off[t] * L::ROW;
+      v[t] = vals0 + at + p.off[t] * L::ES;
     }
 #pragma unroll
     for (int i = 0; i < L::EACH; ++i) {
@@ -143,12 +166,11 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
       lane_load_to_lds(base + rel[i], lds0 + stage * 2 * L::TILE + u * 1024);
     }
   };
-  const int blk0 = key_begin & ~(BLOCK_KEYS - 1);
   const int count = key_end > key_begin ? (key_end - blk0 + BLOCK_KEYS - 1) / BLOCK_KEYS : 0;
 #pragma unroll
   for (int i = 0; i < L::STAGES - 1; ++i)
-    if (i < count) issue(i, find(blk0 + i * BLOCK_KEYS));
-  Places next = find(blk0 + (L::STAGES - 1) * BLOCK_KEYS);     // pages are looked up a block before their loads
+    if (i < count) issue(i, find());
+  Places next = find();                                     // pages are looked up a block before their loads
 
   // ---- the wave's columns
   int limit[CT];                                            // keys that the lane's column sees end here
@@ -201,59 +223,89 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
   }
   auto key_at = [&](int blk, int j) { return HALF ? blk + 8 * kb + j : blk + 16 * (j >> 2) + 4 * kb + (j & 3); };
 
-  auto compute = [&](const char* stage, int blk) {
-    // ---- scores of 32 keys x 16 CT columns
-    f32x4 S[CT][2];
+  // NT: the wave's tiles that hold columns, known where this is compiled: with a branch around every product nothing overlaps
+  auto compute = [&](const char* stage, int blk, auto nt) {
+    constexpr int NT = decltype(nt)::value;
+    // ---- scores of 32 keys x 16 NT columns
+    f32x4 S[NT][2];
+    {
+      Frag a[2][QS];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t) {
+        const int r = HALF ? 8 * (col >> 2) + 4 * t + (col & 3) : 16 * t + col;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) S[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int r = HALF ? 8 * (col >> 2) + 4 * t + (col & 3) : 16 * t + col;
-#pragma unroll
-      for (int s = 0; s < QS; ++s) {
-        Frag a;
-        const bool beyond = HALF && D % 32 != 0 && s == KS - 1 && kb >= 2;      // the last step of 32 dims is half empty
-        a.q = *reinterpret_cast<const uint4*>(stage + r * L::ROW + (((beyond ? 0 : 4 * s + kb)) ^ L::key_turn(r)) * 16);
-        if (beyond) a.q = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          if (ct >= tiles) continue;
-          if constexpr (HALF) {
-            S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, qf[ct][s].v, S[ct][t], 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w[j]), __uint_as_float(qf[ct][s].w[j]), S[ct][t], 0, 0, 0);
-          }
+        for (int s = 0; s < QS; ++s) {
+          const bool beyond = HALF && D % 32 != 0 && s == KS - 1 && kb >= 2;      // the last step of 32 dims is half empty
+          a[t][s].q = *reinterpret_cast<const uint4*>(stage + r * L::ROW + (((beyond ? 0 : 4 * s + kb)) ^ L::key_turn(r)) * 16);
+          if (beyond) a[t][s].q = make_uint4(0, 0, 0, 0);
         }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) S[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < QS; ++s)
+#pragma unroll
+        for (int j = 0; j < (HALF ? 1 : 4); ++j)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int ct = 0; ct < NT; ++ct) {
+              if constexpr (HALF) S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][s].v, qf[ct][s].v, S[ct][t], 0, 0, 0);
+              else S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[t][s].w[j]), __uint_as_float(qf[ct][s].w[j]), S[ct][t], 0, 0, 0);
+            }
+    }
+    // the values of the block, asked for before the weights are known
+    const char* vals = stage + L::TILE;
+    constexpr int VF = HALF ? DT : 2 * DT;
+    Frag va[VF];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int d = dt * 16 + col;
+      if constexpr (HALF) {
+        va[dt].q = *reinterpret_cast<const uint4*>(vals + ((kb >> 1) * D + d) * L::VROW + ((kb & 1) ^ L::value_turn(d)) * 16);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          va[2 * dt + t].q = *reinterpret_cast<const uint4*>(vals + (t * D + d) * L::VROW + (kb ^ L::value_turn(d)) * 16);
       }
     }
     // ---- online softmax, one column a lane's; the maximum follows only when it has grown by more than 2^8, which keeps the sums
     // as far from overflow as they need be and leaves most blocks without a rescaling
-    const bool partial = blk < key_begin || blk + BLOCK_KEYS > least;
-    float p[CT][8];
+    if (blk < key_begin || blk + BLOCK_KEYS > least) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      if (ct >= tiles) continue;
-      if (partial) {
+      for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = key_at(blk, j);
           if (key < key_begin || key >= limit[ct]) S[ct][j >> 2][j & 3] = -INFINITY;
         }
-      }
-      float mx = S[ct][0][0];
+    }
+    float mx[NT];
+    bool grown = false;
 #pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, S[ct][j >> 2][j & 3]);
-      mx = quad_max(mx) * scale_log2;
-      if (__any(mx > m[ct] + 8.f)) {
-        const float m_new = fmaxf(m[ct], mx);
+    for (int ct = 0; ct < NT; ++ct) {
+      mx[ct] = S[ct][0][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mx[ct] = fmaxf(mx[ct], S[ct][j >> 2][j & 3]);
+      mx[ct] = quad_max(mx[ct]) * scale_log2;
+      grown |= mx[ct] > m[ct] + 8.f;
+    }
+    if (__any(grown)) {
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        const float m_new = fmaxf(m[ct], mx[ct]);
         const float alpha = m[ct] == -INFINITY ? 0.f : fast_exp2(m[ct] - m_new);
         m[ct] = m_new;
         l[ct] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) O[ct][dt] *= alpha;
       }
+    }
+    float p[NT][8];
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
       const float base = m[ct] == -INFINITY ? 0.f : m[ct];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -261,74 +313,65 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
         l[ct] += p[ct][j];
       }
     }
-    // ---- values
-    const bool stale = blk < key_begin || blk + BLOCK_KEYS > most;      // some keys no column sees: 0 * (whatever is there) must not reach a sum
-    const char* vals = stage + L::TILE;
-    if constexpr (HALF) {
-      Frag pb[CT];
+    // ---- values; 0 * (whatever is in slots that no column sees) must not reach a sum
+    if (blk < key_begin || blk + BLOCK_KEYS > most) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        if (ct >= tiles) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) pb[ct].w[j] = pack_bf16(p[ct][2 * j], p[ct][2 * j + 1]);
-      }
-      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-      if (stale) {
+      for (int f = 0; f < VF; ++f)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int key = key_at(blk, 2 * j);
-          keep[j] = (key >= key_begin && key < most ? 0x0000FFFFu : 0u) | (key + 1 >= key_begin && key + 1 < most ? 0xFFFF0000u : 0u);
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const int d = dt * 16 + col;
-        Frag va;
-        va.q = *reinterpret_cast<const uint4*>(vals + ((kb >> 1) * D + d) * L::VROW + ((kb & 1) ^ L::value_turn(d)) * 16);
-        if (stale) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) va.w[j] &= keep[j];
-        }
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          if (ct < tiles) O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pb[ct].v, O[ct][dt], 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const int d = dt * 16 + col;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          Frag va;
-          va.q = *reinterpret_cast<const uint4*>(vals + (t * D + d) * L::VROW + (kb ^ L::value_turn(d)) * 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key_at(blk, 4 * t + i);
-            float a = __uint_as_float(va.w[i]);
-            if (stale && (key < key_begin || key >= most)) a = 0.f;
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-              if (ct < tiles) O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, p[ct][4 * t + i], O[ct][dt], 0, 0, 0);
+          if constexpr (HALF) {
+            const int key = key_at(blk, 2 * j);
+            va[f].w[j] &= (key >= key_begin && key < most ? 0x0000FFFFu : 0u) | (key + 1 >= key_begin && key + 1 < most ? 0xFFFF0000u : 0u);
+          } else {
+            const int key = key_at(blk, 4 * (f & 1) + j);
+            if (key < key_begin || key >= most) va[f].w[j] = 0;
           }
         }
-      }
+    }
+    if constexpr (HALF) {
+      Frag pb[NT];
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pb[ct].w[j] = pack_bf16(p[ct][2 * j], p[ct][2 * j + 1]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt].v, pb[ct].v, O[ct][dt], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int ct = 0; ct < NT; ++ct)
+            O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va[2 * dt + (j >> 2)].w[j & 3]), p[ct][j], O[ct][dt], 0, 0, 0);
     }
   };
 
-  for (int n = 0; n < count; ++n) {
-    // block n has landed for every wave, and nobody reads the stage of block n - 1 any more
-    if (n + L::STAGES - 1 <= count) MIE_VMCNT((L::STAGES - 2) * L::EACH);
-    else MIE_VMCNT(0);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (n + L::STAGES - 1 < count) {
-      issue((n + L::STAGES - 1) % L::STAGES, next);
-      next = find(blk0 + (n + L::STAGES) * BLOCK_KEYS);
+  // one loop for each number of tiles a wave may have (waves of a workgroup meet at barriers, whichever loop they are in)
+  auto walk = [&](auto nt) {
+    int stage = 0, fill = L::STAGES - 1;                    // where block n is, where block n + STAGES - 1 goes
+    for (int n = 0; n < count; ++n) {
+      // block n has landed for every wave, and nobody reads the stage of block n - 1 any more
+      if (n + L::STAGES - 1 <= count) MIE_VMCNT((L::STAGES - 2) * L::EACH);
+      else MIE_VMCNT(0);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (n + L::STAGES - 1 < count) {
+        issue(fill, next);
+        next = find();
+      }
+      if constexpr (decltype(nt)::value > 0) compute(lds + stage * 2 * L::TILE, blk0 + n * BLOCK_KEYS, nt);
+      fill = stage;
+      stage = stage + 1 < L::STAGES ? stage + 1 : 0;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    if (tiles > 0) compute(lds + (n % L::STAGES) * 2 * L::TILE, blk0 + n * BLOCK_KEYS);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
+  };
+  if (CT == 2 && tiles == 2) walk(std::integral_constant<int, CT>());
+  else if (tiles > 0) walk(std::integral_constant<int, 1>());
+  else walk(std::integral_constant<int, 0>());
 
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -362,23 +405,23 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
   }
 }
 
-// The parts of a row and query head, one wave each: weights from the log-sum-exps, then the parts' outputs, eight asked for together.
+// The parts of a row and query head: weights from the log-sum-exps, then the parts' outputs, eight asked for together by each of the
+// workgroup's waves, which take the parts in turn and meet in the LDS.
 template <typename T>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(WAVES * 64)
 join_parts_kernel(const float* __restrict__ o_part, const float* __restrict__ lse_part, T* __restrict__ out,
                   const int* __restrict__ row_parts, int Hq, float sink_log2, const float* __restrict__ head_sinks) {
   constexpr int DL = (D + 63) / 64, AHEAD = 8;
-  const int r = blockIdx.x / Hq, head = blockIdx.x - r * Hq, lane = threadIdx.x;
+  __shared__ float s_acc[WAVES][DL * 64], s_m[WAVES], s_w[WAVES];
+  const int r = blockIdx.x / Hq, head = blockIdx.x - r * Hq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int waves = blockDim.x >> 6;
   const int first = row_parts[r], n = row_parts[r + 1] - first;
   if (n == 1) return;                                       // written by its only item
-  float M = -INFINITY;
-  for (int j = lane; j < n; j += 64) M = fmaxf(M, lse_part[(size_t)(first + j) * Hq + head]);
-  M = wave_max(M);
-  float acc[DL], W = 0.f;
+  float acc[DL], W = 0.f, M = -INFINITY;
 #pragma unroll
   for (int i = 0; i < DL; ++i) acc[i] = 0.f;
-  for (int j0 = 0; j0 < n; j0 += AHEAD) {
-    float w[AHEAD], v[AHEAD][DL];
+  for (int j0 = wave * AHEAD; j0 < n; j0 += waves * AHEAD) {
+    float w[AHEAD], v[AHEAD][DL], most = M;
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const size_t at = (size_t)(first + (j0 + j < n ? j0 + j : n - 1)) * Hq + head;
@@ -388,10 +431,35 @@ join_parts_kernel(const float* __restrict__ o_part, const float* __restrict__ ls
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const float x = j0 + j >= n || w[j] == -INFINITY ? 0.f : exp2f(w[j] - M);
+      if (j0 + j >= n) w[j] = -INFINITY;
+      most = fmaxf(most, w[j]);
+    }
+    const float f = M == -INFINITY ? 0.f : exp2f(M - most);
+    M = most;
+    W *= f;
+#pragma unroll
+    for (int i = 0; i < DL; ++i) acc[i] *= f;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float x = w[j] == -INFINITY ? 0.f : exp2f(w[j] - M);
       W += x;
 #pragma unroll
       for (int i = 0; i < DL; ++i) acc[i] = fmaf(x, v[j][i], acc[i]);
+    }
+  }
+  if (waves > 1) {
+    if (lane == 0) { s_m[wave] = M; s_w[wave] = W; }
+#pragma unroll
+    for (int i = 0; i < DL; ++i) s_acc[wave][lane + 64 * i] = acc[i];
+    __syncthreads();
+    if (wave > 0) return;
+    for (int w = 1; w < waves; ++w) {
+      const float m2 = s_m[w], most = fmaxf(M, m2);
+      const float f = M == -INFINITY ? 0.f : exp2f(M - most), g = m2 == -INFINITY ? 0.f : exp2f(m2 - most);
+      M = most;
+      W = W * f + s_w[w] * g;
+#pragma unroll
+      for (int i = 0; i < DL; ++i) acc[i] = acc[i] * f + s_acc[w][lane + 64 * i] * g;
     }
   }
   const float sink = head_sinks ? head_sinks[head] * 1.4426950408889634f : sink_log2;
@@ -410,7 +478,7 @@ static int launch_items(const void* q, long q_stride, const void* k_cache, const
                         const int* tables, int max_blocks, int pages, const int* positions, const int* items, int num_items,
                         const int* row_parts, int Hq, int Hkv, int page, float scale, float sink, const float* head_sinks, hipStream_t stream) {
   auto* kernel = shared_attention_kernel<T, CT>;
-  constexpr int lds = Layout<T>::LDS;
+  constexpr int lds = Layout<T, CT>::LDS;
   if (lds > 65536 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, "shared_prefix_attention")) return -1;
   const int q_vec = ((uintptr_t)q & 15) == 0 && (q_stride * (long)sizeof(T)) % 16 == 0;
   hipLaunchKernelGGL(kernel, dim3((unsigned)num_items * Hkv), dim3(WAVES * 64), lds, stream, (const T*)q, q_stride, q_vec,
@@ -421,10 +489,10 @@ static int launch_items(const void* q, long q_stride, const void* k_cache, const
 }
 
 // items [num_items, 8], row_parts [rows + 1]: the plan's; o_part [slots, Hq, D] and lse_part [slots, Hq] hold the partial results of rows
-// with several parts (slot row_parts[r] + part).  join: some row has another number of parts than one.  scale, sink: in units of log2 e.
+// with several parts (slot row_parts[r] + part).  most_parts: the largest number of parts a row has, or 1 if every row has exactly one.  scale, sink: in units of log2 e.
 MIE_EXPORT int mie_shared_attention(const void* q, long q_stride, const void* k_cache, const void* v_cache, void* out, int dtype, float* o_part,
                                     float* lse_part, const int* tables, int max_blocks, int pages, const int* positions, int rows,
-                                    const int* items, int num_items, int column_tiles, const int* row_parts, int join, int Hq, int Hkv,
+                                    const int* items, int num_items, int column_tiles, const int* row_parts, int most_parts, int Hq, int Hkv,
                                     int page, float scale_log2, float sink_log2, const float* head_sinks, hipStream_t stream) {
   if (rows <= 0) return 0;
   if (Hkv < 1 || Hq % Hkv || page < 16 || page % 16 || max_blocks < 1 || pages < 1)
@@ -436,16 +504,19 @@ MIE_EXPORT int mie_shared_attention(const void* q, long q_stride, const void* k_
     int rc;
 #define MIE_ITEMS(T, CT) launch_items<T, CT>(q, q_stride, k_cache, v_cache, out, o_part, lse_part, tables, max_blocks, pages, positions, items, \
                                              num_items, row_parts, Hq, Hkv, page, scale_log2, sink_log2, head_sinks, stream)
-    if (dtype == MIE_BF16) rc = column_tiles == 2 ? MIE_ITEMS(bf16, 2) : MIE_ITEMS(bf16, 1);
-    else rc = column_tiles == 2 ? MIE_ITEMS(float, 2) : MIE_ITEMS(float, 1);
+    constexpr int MOST = mie_shared_most_tiles();
+    if (column_tiles < 1 || column_tiles > MOST) MIE_FAIL("shared_prefix_attention: %d tiles of columns a wave, at most %d", column_tiles, MOST);
+    if (dtype == MIE_BF16) rc = column_tiles == MOST ? MIE_ITEMS(bf16, MOST) : MIE_ITEMS(bf16, 1);
+    else rc = column_tiles == MOST ? MIE_ITEMS(float, MOST) : MIE_ITEMS(float, 1);
     if (rc) return rc;
   }
-  if (join) {
+  if (most_parts != 1) {
+    const int waves = most_parts > 24 ? 4 : most_parts > 8 ? 2 : 1;
     if (dtype == MIE_BF16)
-      hipLaunchKernelGGL(join_parts_kernel<bf16>, dim3((unsigned)rows * Hq), dim3(64), 0, stream, o_part, lse_part, (bf16*)out, row_parts, Hq,
+      hipLaunchKernelGGL(join_parts_kernel<bf16>, dim3((unsigned)rows * Hq), dim3(64 * waves), 0, stream, o_part, lse_part, (bf16*)out, row_parts, Hq,
                          sink_log2, head_sinks);
     else
-      hipLaunchKernelGGL(join_parts_kernel<float>, dim3((unsigned)rows * Hq), dim3(64), 0, stream, o_part, lse_part, (float*)out, row_parts, Hq,
+      hipLaunchKernelGGL(join_parts_kernel<float>, dim3((unsigned)rows * Hq), dim3(64 * waves), 0, stream, o_part, lse_part, (float*)out, row_parts, Hq,
                          sink_log2, head_sinks);
     MIE_CHECK_LAUNCH("shared_prefix_attention");
   }

@@ -41,6 +41,25 @@ def _rows_ok(t: torch.Tensor, what: str) -> None:
                          f"strides {t.stride()}")
 
 
+def _rules_vector(what, name, t, dtype, n, device_index):
+    """The address of one of a LogitRules' vectors.  (One test that is true of what is right: these run once a step and vector.)"""
+    if t is None or t.dtype is not dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.get_device() != device_index:
+        raise ValueError(f"{what}: rules.{name} must be contiguous {dtype} [{n}] on this GPU, not "
+                         f"{None if t is None else (t.dtype, tuple(t.shape), t.stride(), t.device)}")
+    return t.data_ptr()
+
+
+def _rules_table(what, name, t, device_index):
+    """Address, numbers from row to row, rows and columns of one of a LogitRules' tables."""
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != device_index:
+        raise ValueError(f"{what}: rules.{name} must be int32 of two dimensions on this GPU")
+    rows, columns = t.shape
+    ld, inner = t.stride()
+    if (inner != 1 and columns > 1) or (rows > 1 and ld < columns):
+        raise ValueError(f"{what}: rules.{name} must have unit inner stride and rows that do not overlap")
+    return t.data_ptr(), max(ld, columns), rows, columns
+
+
 class ProjectionSums:
     """The q/k/v projection of a step as float32 sums [splits, tokens, (Hq + 2 Hkv) D], not yet added up, rotated
     or written to the cache (operands checked).  ``finish()`` does that in a kernel of its own and gives q
@@ -81,6 +100,7 @@ class HipBackend(KernelBackend):
         if not torch.cuda.is_available():
             raise RuntimeError("no GPU visible to torch: the engine needs an MI355X (gfx950)")
         self._libs = {}
+        self._rule_slices = {}      # slices that choosing under rules cuts a row into, by rows and vocabulary
         self._zeros = None          # 256 zero bytes on the device, what masked loads of grouped products read
         self._lt_workspace = None   # device memory the library's product kernels may use
         self._lt_rows = set()       # row counts whose library products get their kernel chosen by timing (prefer_rows)
@@ -1998,7 +2018,7 @@ class HipBackend(KernelBackend):
         library.check(lib, lib.mie_shared_attention(
             qkv.data_ptr(), qkv.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _code(qkv.dtype), at,
             None if at is None else at + 4 * plan.num_parts * Hq * D, bt.data_ptr(), bt.shape[1], k_cache.shape[0], step.positions.data_ptr(), T,
-            plan.items.data_ptr(), plan.num_items, plan.column_tiles, plan.row_parts.data_ptr(), int(plan.join), Hq, Hkv, page,
+            plan.items.data_ptr(), plan.num_items, plan.column_tiles, plan.row_parts.data_ptr(), plan.most_parts, Hq, Hkv, page,
             float(scale) * self.LOG2_E, sink_log2, _ptr(head_sinks), self._stream()))
         return out
 
@@ -2034,42 +2054,31 @@ class HipBackend(KernelBackend):
     def _rules_arguments(self, what, rules, R, V):
         """What the kernels of csrc/logit_rules.hip take of a LogitRules, checked."""
         dev = self._device_index
-
-        def vector(name, dtype, n=R):
-            t = getattr(rules, name)
-            if t is None:
-                raise ValueError(f"{what}: rules without {name}")
-            if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.stride(0) != 1 and n > 1 or t.get_device() != dev:
-                raise ValueError(f"{what}: rules.{name} must be contiguous {dtype} [{n}] on this GPU")
-            return t.data_ptr()
-
-        def table(name):
-            t = getattr(rules, name)
-            if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1 or t.get_device() != dev:
-                raise ValueError(f"{what}: rules.{name} must be int32 with unit inner stride, of two dimensions, on this GPU")
-            if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-                raise ValueError(f"{what}: rules.{name} has rows that overlap")
-            return t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[0], t.shape[1]
-
         i32, f32 = torch.int32, torch.float32
-        args = [None, 0, 0, 0, None, None, None, None, None, None, None, None, None, 0, None, 0, 0, None]
+        history = bias_starts = masks = 0
+        slots = most = history_ld = biases = mask_ld = num_masks = 0
+        slot = length = prompt = repetition = presence = frequency = bias_tokens = bias_values = mask_rows = 0
         if rules.history is not None:
-            args[0:4] = table("history")
-            args[4:10] = (vector("slots", i32), vector("lengths", i32), vector("prompt_lengths", i32), vector("repetition", f32),
-                          vector("presence", f32), vector("frequency", f32))
-            if args[0] == 0:        # a history without numbers: nobody has a text
-                args[0] = None
+            history, history_ld, slots, most = _rules_table(what, "history", rules.history, dev)
+            slot = _rules_vector(what, "slots", rules.slots, i32, R, dev)
+            length = _rules_vector(what, "lengths", rules.lengths, i32, R, dev)
+            prompt = _rules_vector(what, "prompt_lengths", rules.prompt_lengths, i32, R, dev)
+            repetition = _rules_vector(what, "repetition", rules.repetition, f32, R, dev)
+            presence = _rules_vector(what, "presence", rules.presence, f32, R, dev)
+            frequency = _rules_vector(what, "frequency", rules.frequency, f32, R, dev)
         if rules.bias_starts is not None:
-            n = rules.bias_tokens.shape[0] if rules.bias_tokens is not None else 0
-            args[10:14] = vector("bias_starts", i32, R + 1), vector("bias_tokens", i32, n), vector("bias_values", f32, n), n
+            bias_starts = _rules_vector(what, "bias_starts", rules.bias_starts, i32, R + 1, dev)
+            biases = 0 if rules.bias_tokens is None else rules.bias_tokens.numel()
+            bias_tokens = _rules_vector(what, "bias_tokens", rules.bias_tokens, i32, biases, dev)
+            bias_values = _rules_vector(what, "bias_values", rules.bias_values, f32, biases, dev)
         if rules.masks is not None:
-            at, ld, masks, words = table("masks")
+            masks, mask_ld, num_masks, words = _rules_table(what, "masks", rules.masks, dev)
             if words < (V + 31) // 32:
                 raise ValueError(f"{what}: masks of {words} words for a vocabulary of {V}")
-            args[14:18] = at, ld, masks, vector("mask_rows", i32)
-            if masks == 0:
-                args[14] = None
-        return args
+            mask_rows = _rules_vector(what, "mask_rows", rules.mask_rows, i32, R, dev)
+        # (an address of 0: a table without numbers, which says nothing about any row)
+        return (history, history_ld, slots, most, slot, length, prompt, repetition, presence, frequency, bias_starts, bias_tokens,
+                bias_values, biases, masks, mask_ld, num_masks, mask_rows)
 
     def sample(self, logits, temperatures, seeds, counters, out=None, rules=None):
         self._on_device(logits, temperatures, seeds, counters, out)
@@ -2094,12 +2103,17 @@ class HipBackend(KernelBackend):
             raise ValueError("sample: temperatures, seeds and counters must be contiguous")
         args = self._rules_arguments("sample", rules, R, V)
         lib = self.lib("logit_rules")
-        slices = -(-V // lib.mie_rules_slice(R, V)) if V else 1
-        best = torch.empty((2, R, slices), dtype=torch.int32, device=logits.device) if slices > 1 else None
-        at = best.data_ptr() if best is not None else None
+        if (R, V) not in self._rule_slices:
+            if len(self._rule_slices) >= 4096:
+                self._rule_slices.clear()
+            self._rule_slices[(R, V)] = lib.mie_rules_slices(R, V)
+        slices, best = self._rule_slices[(R, V)], 0
+        if slices > 1:                  # every slice's best, value and token
+            workspace = torch.empty(2 * R * slices, dtype=torch.int32, device=logits.device)
+            best = workspace.data_ptr()
         library.check(lib, lib.mie_choose_by_rules(
-            logits.data_ptr(), max(logits.stride(0), V), *args, temperatures.data_ptr(), seeds.data_ptr(), counters.data_ptr(), at,
-            None if at is None else at + 4 * R * slices, out.data_ptr(), R, V, self._stream()))
+            logits.data_ptr(), max(logits.stride(0), V), *args, temperatures.data_ptr(), seeds.data_ptr(), counters.data_ptr(), best,
+            best + 4 * R * slices, out.data_ptr(), R, V, self._stream()))
         return out
 
     def adjust_logits(self, logits, rules, out=None):
@@ -2109,7 +2123,7 @@ class HipBackend(KernelBackend):
             out = torch.empty((R, V), dtype=torch.float32, device=logits.device)
         elif out.dtype != torch.float32 or tuple(out.shape) != (R, V) or out.stride(1) != 1 or (R > 1 and out.stride(0) < V):
             raise ValueError(f"adjust_logits: out must be float32 [{R}, {V}] with unit inner stride and rows that do not overlap")
-        if R and (out.data_ptr(), out.stride(0)) != (logits.data_ptr(), logits.stride(0)):
+        if out is not logits and R and (out.data_ptr(), out.stride(0)) != (logits.data_ptr(), logits.stride(0)):
             span = lambda t: (t.data_ptr(), t.data_ptr() + ((R - 1) * t.stride(0) + V) * 4)     # noqa: E731
             (a, b), (c, d) = span(out), span(logits)
             if a < d and c < b:

@@ -119,7 +119,7 @@ register_kernel_module("sampling", {
 })
 _rules = [P, L, I, I, P, P, P, P, P, P, P, P, P, I, P, L, I, P]
 register_kernel_module("logit_rules", {
-    "mie_rules_slice": [I, I],
+    "mie_rules_slices": [I, I],
     "mie_adjust_logits": [P, L, *_rules, P, L, I, I, P],
     "mie_choose_by_rules": [P, L, *_rules, P, P, P, P, P, P, I, I, P],
     "mie_record_tokens": [P, L, I, I, P, P, P, I, P, P, I, P, I, P],

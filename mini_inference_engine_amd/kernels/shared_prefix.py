@@ -12,6 +12,8 @@ import torch
 
 TILE = 64               # columns that a workgroup's four waves take with one tile of 16 each
 BLOCK_KEYS = 32
+import os
+ORDER = os.environ.get('XORDER')
 
 
 class SharedPrefixPlan:
@@ -19,7 +21,7 @@ class SharedPrefixPlan:
     most keys each row has while the plan is used (its position + 1, or more: a plan holds for as many steps as its rows and
     shared keys stay and their contexts suffice).  Made once a step, or once for many, and used by every layer of it."""
 
-    def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256):
+    def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256, least_keys=64, per_unit=2):
         contexts = [int(c) for c in contexts]
         groups = [(int(n), int(k)) for n, k in groups]
         if num_kv_heads < 1 or num_q_heads % num_kv_heads:
@@ -45,14 +47,14 @@ class SharedPrefixPlan:
                     work.append((r, G, k, contexts[r]))
             first += n
         widest = max((w[1] for w in work), default=1)
-        self.column_tiles = 2 if widest > TILE else 1
+        self.column_tiles = 2 if widest > TILE and head_dim <= 128 else 1
         wide = TILE * self.column_tiles
         tiles = [-(-w[1] // wide) for w in work]
         total = sum(t * (w[3] - w[2]) for w, t in zip(work, tiles)) * num_kv_heads
-        # keys an item: four items a compute unit, and no less than 256 (an item's start and its partial result cost about as much)
-        most = max(256, -(-total // (4 * units) // BLOCK_KEYS) * BLOCK_KEYS)
+        # keys an item: two items a compute unit, and no less than 64 (an item's start and its partial result cost about as much)
+        most = max(least_keys, -(-total // (per_unit * units) // BLOCK_KEYS) * BLOCK_KEYS)
         parts = np.zeros(self.num_rows, dtype=np.int64)
-        items = []
+        items, several, pieces_of = [], [], []
         for (row, columns, begin, end), t in zip(work, tiles):
             pieces = -(-(end - begin) // most)
             size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
@@ -61,14 +63,25 @@ class SharedPrefixPlan:
             while at < end:
                 # cuts lie on whole blocks of the cache, so that no block is read twice
                 to = end if end - at <= size else (at + size) // BLOCK_KEYS * BLOCK_KEYS
-                items += [(row, columns, c * wide, at, to, int(parts[row]), 0, 0) for c in range(t)]
+                if rows > 1:
+                    pieces_of += [(pieces_of[-1] if pieces_of else 0) + 1] * t
+                (several if rows > 1 else items).extend((row, columns, c * wide, at, to, int(parts[row]), 0, 0) for c in range(t))
                 parts[row:row + rows] += 1
                 at = to
+        # items of many columns compute, items of one row read: spread among one another, so that a compute unit does both at once
+        if several and items and not ORDER:
+            # (the tiles of columns that read the same keys stay together: the keys then come from the memory once)
+            place = np.concatenate([np.asarray(pieces_of) / pieces_of[-1], np.arange(len(items)) / len(items)])
+            both = several + items
+            items = [both[i] for i in np.argsort(place, kind="stable")]
+        else:
+            items = several + items if ORDER != 'own' else items + several
         self.num_items = len(items)
         starts = np.zeros(self.num_rows + 1, dtype=np.int32)
         np.cumsum(parts, out=starts[1:])
         self.num_parts = int(starts[-1])
-        self.join = bool((parts != 1).any())
+        self.most_parts = 1 if (parts == 1).all() else max(2, int(parts.max()))      # 1: every row has one, nothing to join
+        self.join = self.most_parts != 1
         packed = np.concatenate([np.asarray(items, dtype=np.int32).reshape(-1), starts])
         data = torch.from_numpy(packed)
         if torch.device(device).type == "cuda":
