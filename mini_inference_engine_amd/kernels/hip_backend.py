@@ -42,9 +42,9 @@ def _rows_ok(t: torch.Tensor, what: str) -> None:
 
 
 def _rules_vector(what, name, t, dtype, n, device_index):
-    """The address of one of a LogitRules' vectors.  (One test that is true of what is right: these run once a step and vector.)"""
+    """The address of a vector, one of a LogitRules' or another small one.  (One test that is true of what is right: these run once a step and vector.)"""
     if t is None or t.dtype is not dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.get_device() != device_index:
-        raise ValueError(f"{what}: rules.{name} must be contiguous {dtype} [{n}] on this GPU, not "
+        raise ValueError(f"{what}: {name} must be contiguous {dtype} [{n}] on this GPU, not "
                          f"{None if t is None else (t.dtype, tuple(t.shape), t.stride(), t.device)}")
     return t.data_ptr()
 
@@ -52,11 +52,11 @@ def _rules_vector(what, name, t, dtype, n, device_index):
 def _rules_table(what, name, t, device_index):
     """Address, numbers from row to row, rows and columns of one of a LogitRules' tables."""
     if t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != device_index:
-        raise ValueError(f"{what}: rules.{name} must be int32 of two dimensions on this GPU")
+        raise ValueError(f"{what}: {name} must be int32 of two dimensions on this GPU")
     rows, columns = t.shape
     ld, inner = t.stride()
     if (inner != 1 and columns > 1) or (rows > 1 and ld < columns):
-        raise ValueError(f"{what}: rules.{name} must have unit inner stride and rows that do not overlap")
+        raise ValueError(f"{what}: {name} must have unit inner stride and rows that do not overlap")
     return t.data_ptr(), max(ld, columns), rows, columns
 
 
@@ -100,6 +100,7 @@ class HipBackend(KernelBackend):
         if not torch.cuda.is_available():
             raise RuntimeError("no GPU visible to torch: the engine needs an MI355X (gfx950)")
         self._libs = {}
+        self._shared_libs = {}      # of attention over shared keys, by head size
         self._rule_slices = {}      # slices that choosing under rules cuts a row into, by rows and vocabulary
         self._zeros = None          # 256 zero bytes on the device, what masked loads of grouped products read
         self._lt_workspace = None   # device memory the library's product kernels may use
@@ -2001,25 +2002,29 @@ class HipBackend(KernelBackend):
     def shared_prefix_attention(self, qkv, num_q_heads, num_kv_heads, head_dim, k_cache, v_cache, group, step, scale, plan, sink=None):
         Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim
         T, page, bt = self._check_shared(qkv, Hq, Hkv, D, k_cache, v_cache, group, step, scale, plan)
-        head_sinks, sink_log2 = None, float("-inf")
+        dev = self._device_index
+        for t in (qkv, k_cache, v_cache, bt, step.positions, plan.items):
+            if t.get_device() != dev:
+                raise ValueError(f"shared_prefix_attention: a tensor on {t.device}")
+        head_sinks, sink_log2 = 0, float("-inf")
         if isinstance(sink, torch.Tensor):
-            self._on_device(sink)
-            self._f32_vector(sink, Hq, "shared_prefix_attention: sinks")
-            head_sinks = sink
+            head_sinks = _rules_vector("shared_prefix_attention", "sink", sink, torch.float32, Hq, dev)
         elif sink is not None:
             sink_log2 = float(sink) * self.LOG2_E
-        self._on_device(qkv, k_cache, v_cache, bt, step.positions, plan.items)
-        lib = self.lib("shared_attention", (f"-DHEAD_DIM={D}",))
+        lib = self._shared_libs.get(D)
+        if lib is None:
+            lib = self._shared_libs[D] = self.lib("shared_attention", (f"-DHEAD_DIM={D}",))
         out = torch.empty((T, Hq * D), dtype=qkv.dtype, device=qkv.device)
-        parts = None
+        at = 0
         if plan.join:               # partial outputs, then their log-sum-exps
             parts = torch.empty(plan.num_parts * Hq * (D + 1), dtype=torch.float32, device=qkv.device)
-        at = None if parts is None else parts.data_ptr()
+            at = parts.data_ptr()
+        items, row_parts = plan.addresses
         library.check(lib, lib.mie_shared_attention(
             qkv.data_ptr(), qkv.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _code(qkv.dtype), at,
-            None if at is None else at + 4 * plan.num_parts * Hq * D, bt.data_ptr(), bt.shape[1], k_cache.shape[0], step.positions.data_ptr(), T,
-            plan.items.data_ptr(), plan.num_items, plan.column_tiles, plan.row_parts.data_ptr(), plan.most_parts, Hq, Hkv, page,
-            float(scale) * self.LOG2_E, sink_log2, _ptr(head_sinks), self._stream()))
+            at + 4 * plan.num_parts * Hq * D, bt.data_ptr(), bt.shape[1], k_cache.shape[0], step.positions.data_ptr(), T,
+            items, plan.num_items, plan.column_tiles, row_parts, plan.most_parts, Hq, Hkv, page,
+            scale * self.LOG2_E, sink_log2, head_sinks, self._stream()))
         return out
 
     LOG2_E = 1.4426950408889634
@@ -2081,6 +2086,8 @@ class HipBackend(KernelBackend):
                 bias_values, biases, masks, mask_ld, num_masks, mask_rows)
 
     def sample(self, logits, temperatures, seeds, counters, out=None, rules=None):
+        if rules is not None:
+            return self._choose_by_rules(logits, temperatures, seeds, counters, out, rules)
         self._on_device(logits, temperatures, seeds, counters, out)
         R, V = self._check_logits("sample", logits)
         if (temperatures.dtype, seeds.dtype, counters.dtype) != (torch.float32, torch.int64, torch.int32):
@@ -2091,17 +2098,23 @@ class HipBackend(KernelBackend):
             out = torch.empty(R, dtype=torch.int32, device=logits.device)
         elif out.dtype != torch.int32 or tuple(out.shape) != (R,) or not out.is_contiguous():
             raise ValueError(f"sample: out must be contiguous int32 [{R}]")
-        if rules is not None:
-            return self._choose_by_rules(logits, temperatures, seeds, counters, out, rules, R, V)
         lib = self.lib("sampling")
         library.check(lib, lib.mie_sample(_ptr(logits), logits.stride(0), _ptr(temperatures), _ptr(seeds),
                                           _ptr(counters), _ptr(out), R, V, self._stream()))
         return out
 
-    def _choose_by_rules(self, logits, temperatures, seeds, counters, out, rules, R, V):
-        if not (temperatures.is_contiguous() and seeds.is_contiguous() and counters.is_contiguous()):
-            raise ValueError("sample: temperatures, seeds and counters must be contiguous")
+    def _choose_by_rules(self, logits, temperatures, seeds, counters, out, rules):
+        R, V = self._check_logits("sample", logits)
+        dev, i32 = self._device_index, torch.int32
+        if logits.get_device() != dev:
+            raise ValueError(f"sample: logits on {logits.device}")
+        t = _rules_vector("sample", "temperatures", temperatures, torch.float32, R, dev)
+        s = _rules_vector("sample", "seeds", seeds, torch.int64, R, dev)
+        c = _rules_vector("sample", "counters", counters, i32, R, dev)
         args = self._rules_arguments("sample", rules, R, V)
+        if out is None:
+            out = torch.empty(R, dtype=i32, device=logits.device)
+        o = _rules_vector("sample", "out", out, i32, R, dev)
         lib = self.lib("logit_rules")
         if (R, V) not in self._rule_slices:
             if len(self._rule_slices) >= 4096:
@@ -2112,13 +2125,14 @@ class HipBackend(KernelBackend):
             workspace = torch.empty(2 * R * slices, dtype=torch.int32, device=logits.device)
             best = workspace.data_ptr()
         library.check(lib, lib.mie_choose_by_rules(
-            logits.data_ptr(), max(logits.stride(0), V), *args, temperatures.data_ptr(), seeds.data_ptr(), counters.data_ptr(), best,
-            best + 4 * R * slices, out.data_ptr(), R, V, self._stream()))
+            logits.data_ptr(), logits.stride(0) if R > 1 else V, *args, t, s, c, best,
+            best + 4 * R * slices, o, R, V, self._stream()))
         return out
 
     def adjust_logits(self, logits, rules, out=None):
-        self._on_device(logits, out)
         R, V = self._check_logits("adjust_logits", logits)
+        if logits.get_device() != self._device_index or (out is not None and out.get_device() != self._device_index):
+            raise ValueError("adjust_logits: logits and out belong on this GPU")
         if out is None:
             out = torch.empty((R, V), dtype=torch.float32, device=logits.device)
         elif out.dtype != torch.float32 or tuple(out.shape) != (R, V) or out.stride(1) != 1 or (R > 1 and out.stride(0) < V):
@@ -2130,8 +2144,8 @@ class HipBackend(KernelBackend):
                 raise ValueError("adjust_logits: out is the logits themselves or apart from them")
         args = self._rules_arguments("adjust_logits", rules, R, V)
         lib = self.lib("logit_rules")
-        library.check(lib, lib.mie_adjust_logits(logits.data_ptr(), max(logits.stride(0), V), *args, out.data_ptr(), max(out.stride(0), V),
-                                                 R, V, self._stream()))
+        library.check(lib, lib.mie_adjust_logits(logits.data_ptr(), logits.stride(0) if R > 1 else V, *args, out.data_ptr(),
+                                                 out.stride(0) if R > 1 else V, R, V, self._stream()))
         return out
 
     def record_tokens(self, history, step):

@@ -12,8 +12,6 @@ import torch
 
 TILE = 64               # columns that a workgroup's four waves take with one tile of 16 each
 BLOCK_KEYS = 32
-import os
-ORDER = os.environ.get('XORDER')
 
 
 class SharedPrefixPlan:
@@ -54,7 +52,7 @@ class SharedPrefixPlan:
         # keys an item: two items a compute unit, and no less than 64 (an item's start and its partial result cost about as much)
         most = max(least_keys, -(-total // (per_unit * units) // BLOCK_KEYS) * BLOCK_KEYS)
         parts = np.zeros(self.num_rows, dtype=np.int64)
-        items, several, pieces_of = [], [], []
+        items, several = [], []
         for (row, columns, begin, end), t in zip(work, tiles):
             pieces = -(-(end - begin) // most)
             size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
@@ -63,19 +61,12 @@ class SharedPrefixPlan:
             while at < end:
                 # cuts lie on whole blocks of the cache, so that no block is read twice
                 to = end if end - at <= size else (at + size) // BLOCK_KEYS * BLOCK_KEYS
-                if rows > 1:
-                    pieces_of += [(pieces_of[-1] if pieces_of else 0) + 1] * t
                 (several if rows > 1 else items).extend((row, columns, c * wide, at, to, int(parts[row]), 0, 0) for c in range(t))
                 parts[row:row + rows] += 1
                 at = to
-        # items of many columns compute, items of one row read: spread among one another, so that a compute unit does both at once
-        if several and items and not ORDER:
-            # (the tiles of columns that read the same keys stay together: the keys then come from the memory once)
-            place = np.concatenate([np.asarray(pieces_of) / pieces_of[-1], np.arange(len(items)) / len(items)])
-            both = several + items
-            items = [both[i] for i in np.argsort(place, kind="stable")]
-        else:
-            items = several + items if ORDER != 'own' else items + several
+        # the longest first: items of many columns take several times what those of one row do (256 rows behind 8,192 keys: the two kinds
+        # spread among one another 256 us, these first 182)
+        items = several + items
         self.num_items = len(items)
         starts = np.zeros(self.num_rows + 1, dtype=np.int32)
         np.cumsum(parts, out=starts[1:])
@@ -88,3 +79,4 @@ class SharedPrefixPlan:
             data = data.pin_memory().to(device, non_blocking=True)
         self._data = data
         self.items, self.row_parts = data[:8 * len(items)], data[8 * len(items):]
+        self.addresses = self.items.data_ptr(), self.row_parts.data_ptr()

@@ -320,3 +320,6 @@ def test_refused_results(ops):
     with pytest.raises(ValueError, match="logits"):
         ops.adjust_logits(logits.double(), none)
     assert ops.adjust_logits(logits[:0], none).shape == (0, 64)
+    wide = torch.zeros((1, 64), device="cuda").expand(2, 64)          # rows on top of one another
+    with pytest.raises((ValueError, RuntimeError), match="logits|leading"):
+        ops.adjust_logits(wide, none, out=torch.zeros((2, 64), device="cuda"))
