@@ -17,6 +17,9 @@
 #include <type_traits>
 
 constexpr int WAVES = 4;
+#ifndef MIE_STAGES32
+#define MIE_STAGES32 2
+#endif
 // Tiles of 16 columns a wave: two, as far as their outputs have room in the registers.
 constexpr int mie_shared_most_tiles() { return D <= 128 ? 2 : 1; }
 
@@ -41,17 +44,6 @@ struct SharedItem {
   int unused0, unused1;
 };
 
-#ifndef XST1
-#define XST1 3
-#endif
-#ifndef XST2
-#define XST2 5
-#endif
-template <typename T, int CT> constexpr int stages_of() {
-  if (sizeof(T) == 2) return D <= 32 ? 8 : D <= 64 ? 6 : D <= 128 ? (CT == 2 ? XST2 : XST1) : 3;
-  return D <= 64 ? 4 : D <= 128 ? 3 : 2;
-}
-
 template <typename T, int CT>
 struct Layout {
   static constexpr int ES = sizeof(T);
@@ -59,11 +51,17 @@ struct Layout {
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int TURN = CHUNKS % 8 == 0 ? 7 : CHUNKS % 4 == 0 ? 3 : 1;
   static constexpr int VROW = 16 * ES;                      // bytes of 16 keys' values of one dim
-  static constexpr int TILE = 32 * ROW;                     // keys of a block; values take as much
-  static constexpr int UNITS = 2 * TILE / 1024;             // of a block's loads
+  static constexpr int TILE = BLOCK_KEYS * ROW;             // keys of 32; their values take as much
+  static constexpr int UNITS = 2 * TILE / 1024;             // loads of 1 KB that bring both
   static constexpr int EACH = (UNITS + WAVES - 1) / WAVES;  // a wave's
-  static constexpr int STAGES = stages_of<T, CT>();
-  static constexpr int LDS = STAGES * 2 * TILE;
+  static constexpr bool WHOLE = TILE % 2048 == 0;           // no unit lies across the two halves of 16 keys
+  // A stage: what is waited for and computed at once, two times 32 keys where the LDS has room for it (half the barriers, and twice the
+  // independent work behind each).
+  static constexpr int H = ROW <= 256 ? 2 : 1;
+  static constexpr int KEYS = H * BLOCK_KEYS;
+  static constexpr int STAGE = H * 2 * TILE;
+  static constexpr int STAGES = STAGE <= 8192 ? 6 : STAGE <= 16384 ? 4 : STAGE <= 32768 ? MIE_STAGES32 : 2;
+  static constexpr int LDS = STAGES * STAGE;
   // 16-byte places are turned by what tells the rows apart that are read at once, so that they lie in different banks
   static __device__ __forceinline__ int key_turn(int r) { return (ES == 2 ? (r & 3) | ((r >> 3 & 1) << 2) : r & 7) & TURN; }
   static __device__ __forceinline__ int value_turn(int d) { return ES == 2 ? d >> 2 & 1 : d >> 1 & 3; }
@@ -95,7 +93,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     key_end = seen < key_end ? seen : key_end;
   }
 
-  // ---- the loads: unit u of a block is 1 KB of its keys or values, a wave takes units wave, wave + 4, ..
+  // ---- the loads: unit u of 32 keys is 1 KB of their keys or values, a wave takes units wave, wave + 4, ..
   uint32_t rel[L::EACH];
   bool upper[L::EACH], is_key[L::EACH];
 #pragma unroll
@@ -103,26 +101,27 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     int u = wave + WAVES * i;
     u = u < L::UNITS ? u : L::UNITS - 1;                    // (a wave without a unit of its own repeats the last one)
     int x = u * 1024 + lane * 16;
-    is_key[i] = x < L::TILE;
+    is_key[i] = L::UNITS % (2 * WAVES) == 0 ? i < L::EACH / 2 : u < L::UNITS / 2;
     if (is_key[i]) {
       const int r = x / L::ROW, place = (x - r * L::ROW) / 16;
-      upper[i] = r >= 16;
+      upper[i] = L::UNITS % (4 * WAVES) == 0 ? i >= L::EACH / 4 : L::WHOLE ? u >= L::UNITS / 4 : r >= 16;
       rel[i] = (r & 15) * L::ROW + (place ^ L::key_turn(r)) * 16;
     } else {
       x -= L::TILE;
       const int half = x / (D * L::VROW);
       x -= half * D * L::VROW;
       const int d = x / L::VROW, place = (x - d * L::VROW) / 16;
-      upper[i] = half;
+      upper[i] = L::UNITS % (4 * WAVES) == 0 ? i >= 3 * L::EACH / 4 : L::WHOLE ? u >= 3 * (L::UNITS / 4) : half;
       rel[i] = d * page * L::ES + (place ^ L::value_turn(d)) * 16;
     }
   }
   const auto* table = (const __attribute__((address_space(4))) int*)(uintptr_t)(tables + (size_t)first_row * max_blocks);
   // Where a block's keys lie: its halves of 16 keys are in one page each.  Followed from block to block by additions.
-  const int blk0 = key_begin & ~(BLOCK_KEYS - 1);
+  const int blk0 = key_begin & ~(BLOCK_KEYS - 1);       // 32 and not a stage: a cut lies on any 32 keys
   const uint64_t page_bytes = (uint64_t)(uint32_t)Hkv * page * L::ROW;       // of keys; of values as well
   const char* const keys0 = reinterpret_cast<const char*>(k_cache) + (size_t)kvh * page * L::ROW;
   const char* const vals0 = reinterpret_cast<const char*>(v_cache) + (size_t)kvh * page * L::ROW;
+  const int more_pages = BLOCK_KEYS / page, more_off = BLOCK_KEYS % page;
   int index[2], off[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -136,20 +135,15 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     for (int t = 0; t < 2; ++t) {
       p.pg[t] = table[index[t] < max_blocks ? index[t] : max_blocks - 1];
       p.off[t] = off[t];
-      if (page == 16) {
-        index[t] += 2;
-      } else {
-        off[t] += BLOCK_KEYS;
-        if (off[t] >= page) {
-          off[t] -= page;
-          ++index[t];
-        }
-      }
+      off[t] += more_off;
+      const int turn = off[t] >= page ? 1 : 0;
+      off[t] -= turn * page;
+      index[t] += more_pages + turn;
     }
     return p;
   };
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds;
-  auto issue = [&](int stage, const Places& p) {
+  auto issue = [&](uint32_t to, const Places& p) {
     const char *k[2], *v[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -163,14 +157,29 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
       int u = wave + WAVES * i;
       u = u < L::UNITS ? u : L::UNITS - 1;
       const char* base = is_key[i] ? (upper[i] ? k[1] : k[0]) : (upper[i] ? v[1] : v[0]);
-      lane_load_to_lds(base + rel[i], lds0 + stage * 2 * L::TILE + u * 1024);
+      if constexpr (L::WHOLE) mie_load_to_lds(base, rel[i], to + u * 1024);
+      else lane_load_to_lds(base + rel[i], to + u * 1024);
     }
   };
-  const int count = key_end > key_begin ? (key_end - blk0 + BLOCK_KEYS - 1) / BLOCK_KEYS : 0;
+  const int blocks = key_end > key_begin ? (key_end - blk0 + BLOCK_KEYS - 1) / BLOCK_KEYS : 0, count = (blocks + L::H - 1) / L::H;
+  Places next[L::H];
+  // A stage's last 32 keys may lie beyond the item's: they are not asked for, and what the LDS holds in their place is masked.
+  auto issue_stage = [&](int n, int stage) {
+#pragma unroll
+    for (int h = 0; h < L::H; ++h)
+      if (h == 0 || n * L::H + h < blocks) issue(lds0 + stage * L::STAGE + h * 2 * L::TILE, next[h]);
+  };
+  auto find_stage = [&]() {                                 // pages are looked up a stage before their loads
+#pragma unroll
+    for (int h = 0; h < L::H; ++h) next[h] = find();
+  };
+  find_stage();
 #pragma unroll
   for (int i = 0; i < L::STAGES - 1; ++i)
-    if (i < count) issue(i, find());
-  Places next = find();                                     // pages are looked up a block before their loads
+    if (i < count) {
+      issue_stage(i, i);
+      find_stage();
+    }
 
   // ---- the wave's columns
   int limit[CT];                                            // keys that the lane's column sees end here
@@ -221,14 +230,20 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) O[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  auto key_at = [&](int blk, int j) { return HALF ? blk + 8 * kb + j : blk + 16 * (j >> 2) + 4 * kb + (j & 3); };
+  // key of a lane's j-th score of the h-th 32 keys
+  auto key_at = [&](int blk, int h, int j) {
+    return blk + BLOCK_KEYS * h + (HALF ? 8 * kb + j : 16 * (j >> 2) + 4 * kb + (j & 3));
+  };
 
   // NT: the wave's tiles that hold columns, known where this is compiled: with a branch around every product nothing overlaps
-  auto compute = [&](const char* stage, int blk, auto nt) {
+  // MASKED: some of the stage's keys are hidden from some columns.
+  auto compute = [&](const char* stage, int blk, auto nt, auto masked) {
     constexpr int NT = decltype(nt)::value;
-    // ---- scores of 32 keys x 16 NT columns
-    f32x4 S[NT][2];
-    {
+    constexpr bool MASKED = decltype(masked)::value;
+    // ---- scores of a stage's keys x 16 NT columns
+    f32x4 S[L::H][NT][2];
+#pragma unroll
+    for (int h = 0; h < L::H; ++h) {
       Frag a[2][QS];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -236,14 +251,14 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
           const bool beyond = HALF && D % 32 != 0 && s == KS - 1 && kb >= 2;      // the last step of 32 dims is half empty
-          a[t][s].q = *reinterpret_cast<const uint4*>(stage + r * L::ROW + (((beyond ? 0 : 4 * s + kb)) ^ L::key_turn(r)) * 16);
+          a[t][s].q = *reinterpret_cast<const uint4*>(stage + h * 2 * L::TILE + r * L::ROW + (((beyond ? 0 : 4 * s + kb)) ^ L::key_turn(r)) * 16);
           if (beyond) a[t][s].q = make_uint4(0, 0, 0, 0);
         }
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int ct = 0; ct < NT; ++ct) S[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int ct = 0; ct < NT; ++ct) S[h][ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < QS; ++s)
 #pragma unroll
@@ -252,43 +267,30 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int ct = 0; ct < NT; ++ct) {
-              if constexpr (HALF) S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][s].v, qf[ct][s].v, S[ct][t], 0, 0, 0);
-              else S[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[t][s].w[j]), __uint_as_float(qf[ct][s].w[j]), S[ct][t], 0, 0, 0);
+              if constexpr (HALF) S[h][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][s].v, qf[ct][s].v, S[h][ct][t], 0, 0, 0);
+              else S[h][ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[t][s].w[j]), __uint_as_float(qf[ct][s].w[j]), S[h][ct][t], 0, 0, 0);
             }
     }
-    // the values of the block, asked for before the weights are known
-    const char* vals = stage + L::TILE;
-    constexpr int VF = HALF ? DT : 2 * DT;
-    Frag va[VF];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int d = dt * 16 + col;
-      if constexpr (HALF) {
-        va[dt].q = *reinterpret_cast<const uint4*>(vals + ((kb >> 1) * D + d) * L::VROW + ((kb & 1) ^ L::value_turn(d)) * 16);
-      } else {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          va[2 * dt + t].q = *reinterpret_cast<const uint4*>(vals + (t * D + d) * L::VROW + (kb ^ L::value_turn(d)) * 16);
-      }
-    }
     // ---- online softmax, one column a lane's; the maximum follows only when it has grown by more than 2^8, which keeps the sums
-    // as far from overflow as they need be and leaves most blocks without a rescaling
-    if (blk < key_begin || blk + BLOCK_KEYS > least) {
+    // as far from overflow as they need be and leaves most stages without a rescaling
+    if constexpr (MASKED) {
 #pragma unroll
-      for (int ct = 0; ct < NT; ++ct)
+      for (int h = 0; h < L::H; ++h)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = key_at(blk, j);
-          if (key < key_begin || key >= limit[ct]) S[ct][j >> 2][j & 3] = -INFINITY;
-        }
+        for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = key_at(blk, h, j);
+            if (key < key_begin || key >= limit[ct]) S[h][ct][j >> 2][j & 3] = -INFINITY;
+          }
     }
     float mx[NT];
     bool grown = false;
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      mx[ct] = S[ct][0][0];
+      mx[ct] = S[0][ct][0][0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) mx[ct] = fmaxf(mx[ct], S[ct][j >> 2][j & 3]);
+      for (int j = 1; j < 8 * L::H; ++j) mx[ct] = fmaxf(mx[ct], S[j >> 3][ct][j >> 2 & 1][j & 3]);
       mx[ct] = quad_max(mx[ct]) * scale_log2;
       grown |= mx[ct] > m[ct] + 8.f;
     }
@@ -303,70 +305,95 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
         for (int dt = 0; dt < DT; ++dt) O[ct][dt] *= alpha;
       }
     }
-    float p[NT][8];
 #pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      const float base = m[ct] == -INFINITY ? 0.f : m[ct];
+    for (int h = 0; h < L::H; ++h) {
+      // the values of 32 keys, asked for before the weights are known
+      const char* vals = stage + h * 2 * L::TILE + L::TILE;
+      constexpr int VF = HALF ? DT : 2 * DT;
+      Frag va[VF];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[ct][j] = fast_exp2(fmaf(S[ct][j >> 2][j & 3], scale_log2, -base));
-        l[ct] += p[ct][j];
-      }
-    }
-    // ---- values; 0 * (whatever is in slots that no column sees) must not reach a sum
-    if (blk < key_begin || blk + BLOCK_KEYS > most) {
+      for (int dt = 0; dt < DT; ++dt) {
+        const int d = dt * 16 + col;
+        if constexpr (HALF) {
+          va[dt].q = *reinterpret_cast<const uint4*>(vals + ((kb >> 1) * D + d) * L::VROW + ((kb & 1) ^ L::value_turn(d)) * 16);
+        } else {
 #pragma unroll
-      for (int f = 0; f < VF; ++f)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (HALF) {
-            const int key = key_at(blk, 2 * j);
-            va[f].w[j] &= (key >= key_begin && key < most ? 0x0000FFFFu : 0u) | (key + 1 >= key_begin && key + 1 < most ? 0xFFFF0000u : 0u);
-          } else {
-            const int key = key_at(blk, 4 * (f & 1) + j);
-            if (key < key_begin || key >= most) va[f].w[j] = 0;
-          }
+          for (int t = 0; t < 2; ++t)
+            va[2 * dt + t].q = *reinterpret_cast<const uint4*>(vals + (t * D + d) * L::VROW + (kb ^ L::value_turn(d)) * 16);
         }
-    }
-    if constexpr (HALF) {
-      Frag pb[NT];
+      }
+      float p[NT][8];
 #pragma unroll
-      for (int ct = 0; ct < NT; ++ct)
+      for (int ct = 0; ct < NT; ++ct) {
+        const float base = m[ct] == -INFINITY ? 0.f : m[ct];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pb[ct].w[j] = pack_bf16(p[ct][2 * j], p[ct][2 * j + 1]);
+        for (int j = 0; j < 8; ++j) {
+          p[ct][j] = fast_exp2(fmaf(S[h][ct][j >> 2][j & 3], scale_log2, -base));
+          l[ct] += p[ct][j];
+        }
+      }
+      // 0 * (whatever is in slots that no column sees) must not reach a sum
+      if (MASKED && (blk < key_begin || blk + BLOCK_KEYS * (h + 1) > most)) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+        for (int f = 0; f < VF; ++f)
 #pragma unroll
-        for (int ct = 0; ct < NT; ++ct) O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt].v, pb[ct].v, O[ct][dt], 0, 0, 0);
-    } else {
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (HALF) {
+              const int key = key_at(blk, h, 2 * j);
+              va[f].w[j] &= (key >= key_begin && key < most ? 0x0000FFFFu : 0u) | (key + 1 >= key_begin && key + 1 < most ? 0xFFFF0000u : 0u);
+            } else {
+              const int key = key_at(blk, h, 4 * (f & 1) + j);
+              if (key < key_begin || key >= most) va[f].w[j] = 0;
+            }
+          }
+      }
+      if constexpr (HALF) {
+        Frag pb[NT];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+        for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pb[ct].w[j] = pack_bf16(p[ct][2 * j], p[ct][2 * j + 1]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int ct = 0; ct < NT; ++ct)
-            O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va[2 * dt + (j >> 2)].w[j & 3]), p[ct][j], O[ct][dt], 0, 0, 0);
+          for (int ct = 0; ct < NT; ++ct) O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt].v, pb[ct].v, O[ct][dt], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int ct = 0; ct < NT; ++ct)
+              O[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va[2 * dt + (j >> 2)].w[j & 3]), p[ct][j], O[ct][dt], 0, 0, 0);
+      }
     }
   };
 
   // one loop for each number of tiles a wave may have (waves of a workgroup meet at barriers, whichever loop they are in)
   auto walk = [&](auto nt) {
-    int stage = 0, fill = L::STAGES - 1;                    // where block n is, where block n + STAGES - 1 goes
-    for (int n = 0; n < count; ++n) {
-      // block n has landed for every wave, and nobody reads the stage of block n - 1 any more
-      if (n + L::STAGES - 1 <= count) MIE_VMCNT((L::STAGES - 2) * L::EACH);
-      else MIE_VMCNT(0);
+    int n = 0, stage = 0, fill = L::STAGES - 1;             // where stage n is, where stage n + STAGES - 1 goes
+    auto step = [&](auto masked) {
+      // stage n has landed for every wave, and nobody reads the one before any more
+      if (n + L::STAGES - 1 < count) MIE_VMCNT((L::STAGES - 2) * L::H * L::EACH);
+      else MIE_VMCNT(0);                                    // (the last ones may be shorter)
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       if (n + L::STAGES - 1 < count) {
-        issue(fill, next);
-        next = find();
+        issue_stage(n + L::STAGES - 1, fill);
+        find_stage();
       }
-      if constexpr (decltype(nt)::value > 0) compute(lds + stage * 2 * L::TILE, blk0 + n * BLOCK_KEYS, nt);
+      if constexpr (decltype(nt)::value > 0) compute(lds + stage * L::STAGE, blk0 + n * L::KEYS, nt, masked);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       fill = stage;
       stage = stage + 1 < L::STAGES ? stage + 1 : 0;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      ++n;
+    };
+    const int whole = decltype(nt)::value > 0 ? (least - blk0) / L::KEYS : 0;      // stages before it end where every column sees them
+    while (n < count) {
+      if (n > 0 || blk0 >= key_begin)
+        while (n < whole && n < count) step(std::false_type());
+      if (n < count) step(std::true_type());
     }
   };
   if (CT == 2 && tiles == 2) walk(std::integral_constant<int, CT>());
