@@ -17,9 +17,6 @@
 #include <type_traits>
 
 constexpr int WAVES = 4;
-#ifndef MIE_STAGES32
-#define MIE_STAGES32 2
-#endif
 // Tiles of 16 columns a wave: two, as far as their outputs have room in the registers.
 constexpr int mie_shared_most_tiles() { return D <= 128 ? 2 : 1; }
 
@@ -60,8 +57,14 @@ struct Layout {
   static constexpr int H = ROW <= 256 ? 2 : 1;
   static constexpr int KEYS = H * BLOCK_KEYS;
   static constexpr int STAGE = H * 2 * TILE;
-  static constexpr int STAGES = STAGE <= 8192 ? 6 : STAGE <= 16384 ? 4 : STAGE <= 32768 ? MIE_STAGES32 : 2;
-  static constexpr int LDS = STAGES * STAGE;
+  static constexpr int STAGES = STAGE <= 8192 ? 6 : STAGE <= 16384 ? 4 : 2;
+  // Items of up to 16 columns: each wave takes every fourth 32 keys, by itself, in slots of its own.
+  static constexpr bool APART = WHOLE && ROW <= 512;
+  static constexpr int SLOT = 2 * TILE;
+  static constexpr int SLOTS = STAGES * STAGE / (WAVES * SLOT) > 1 ? 2 : 1;
+  static constexpr int JOIN = WAVES * 16 * (D + 1) * 4;     // the waves' sums, where the slots were
+  static constexpr int LDS = !APART ? STAGES * STAGE : STAGES * STAGE > WAVES * SLOTS * SLOT ? (STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN)
+                                                                                             : (WAVES * SLOTS * SLOT > JOIN ? WAVES * SLOTS * SLOT : JOIN);
   // 16-byte places are turned by what tells the rows apart that are read at once, so that they lie in different banks
   static __device__ __forceinline__ int key_turn(int r) { return (ES == 2 ? (r & 3) | ((r >> 3 & 1) << 2) : r & 7) & TURN; }
   static __device__ __forceinline__ int value_turn(int d) { return ES == 2 ? d >> 2 & 1 : d >> 1 & 3; }
@@ -88,10 +91,16 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
   const int G = Hq / Hkv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kb = lane >> 4;
+  // Keys that no other workgroup reads are loaded with the hint that nobody reads them again: they then push neither the shared keys nor
+  // anything else out of the caches (256 rows behind 8,192 keys 177 -> 150 us, their own 1 to 1,024 keys alone 157 -> 97, 8 rows behind
+  // 30,000 keys 58 -> 35).
+  const bool once = columns <= WAVES * 16 * CT;
   if (columns <= G) {                                       // one row: nothing behind its own key
     const int seen = positions[first_row] + 1;
     key_end = seen < key_end ? seen : key_end;
   }
+
+  const bool apart = L::APART && columns <= 16;             // the waves share out keys, not columns
 
   // ---- the loads: unit u of 32 keys is 1 KB of their keys or values, a wave takes units wave, wave + 4, ..
   uint32_t rel[L::EACH];
@@ -121,15 +130,16 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
   const uint64_t page_bytes = (uint64_t)(uint32_t)Hkv * page * L::ROW;       // of keys; of values as well
   const char* const keys0 = reinterpret_cast<const char*>(k_cache) + (size_t)kvh * page * L::ROW;
   const char* const vals0 = reinterpret_cast<const char*>(v_cache) + (size_t)kvh * page * L::ROW;
-  const int more_pages = BLOCK_KEYS / page, more_off = BLOCK_KEYS % page;
+  const int stride = apart ? WAVES * BLOCK_KEYS : BLOCK_KEYS, blk1 = blk0 + (apart ? wave * BLOCK_KEYS : 0);
+  const int more_pages = stride / page, more_off = stride % page;
   int index[2], off[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    index[t] = (blk0 + 16 * t) / page;
-    off[t] = blk0 + 16 * t - index[t] * page;
+    index[t] = (blk1 + 16 * t) / page;
+    off[t] = blk1 + 16 * t - index[t] * page;
   }
   struct Places { int pg[2], off[2]; };
-  auto find = [&]() {                                       // of the next block in order
+  auto find = [&]() {                                       // of the next block of the wave's
     Places p;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -157,7 +167,10 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
       int u = wave + WAVES * i;
       u = u < L::UNITS ? u : L::UNITS - 1;
       const char* base = is_key[i] ? (upper[i] ? k[1] : k[0]) : (upper[i] ? v[1] : v[0]);
-      if constexpr (L::WHOLE) mie_load_to_lds(base, rel[i], to + u * 1024);
+      if constexpr (L::WHOLE) {
+        if (once) mie_load_to_lds_nt(base, rel[i], to + u * 1024);
+        else mie_load_to_lds(base, rel[i], to + u * 1024);
+      }
       else lane_load_to_lds(base + rel[i], to + u * 1024);
     }
   };
@@ -173,13 +186,55 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
 #pragma unroll
     for (int h = 0; h < L::H; ++h) next[h] = find();
   };
-  find_stage();
+  // a wave's own 32 keys: units of one half of 16 keys, and of values, differ by their place alone
+  constexpr int KL = L::APART ? L::UNITS / 4 : 1;
+  uint32_t koff[KL], voff = 0;
+  auto issue_own = [&](int slot, const Places& p) {
+    const uint32_t to = lds0 + (wave * L::SLOTS + slot) * L::SLOT;
+    const uint32_t half_bytes = L::TILE / 2, dims = 1024 / L::VROW;      // of a unit of values
 #pragma unroll
-  for (int i = 0; i < L::STAGES - 1; ++i)
-    if (i < count) {
-      issue_stage(i, i);
-      find_stage();
+    for (int t = 0; t < 2; ++t) {
+      const uint64_t at = ((uint32_t)p.pg[t] < (uint32_t)pages ? (uint32_t)p.pg[t] : 0u) * page_bytes;
+      const char* k = keys0 + at + p.off[t] * L::ROW;
+#pragma unroll
+      for (int j = 0; j < KL; ++j) mie_load_to_lds_nt(k, koff[j], to + t * half_bytes + j * 1024);
     }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint64_t at = ((uint32_t)p.pg[t] < (uint32_t)pages ? (uint32_t)p.pg[t] : 0u) * page_bytes;
+      const char* v = vals0 + at + p.off[t] * L::ES;
+#pragma unroll
+      for (int j = 0; j < KL; ++j) mie_load_to_lds_nt(v + (size_t)(j * dims) * page * L::ES, voff, to + L::TILE + t * half_bytes + j * 1024);
+    }
+  };
+  const int mine = apart ? (blocks - wave + WAVES - 1) / WAVES : 0;      // 32 keys each
+  Places next_own;
+  if (apart) {
+    if constexpr (L::APART) {
+#pragma unroll
+      for (int j = 0; j < KL; ++j) {
+        const int x = j * 1024 + lane * 16, r = x / L::ROW, place = (x - r * L::ROW) / 16;
+        koff[j] = r * L::ROW + (place ^ L::key_turn(r)) * 16;
+      }
+      const int d = lane * 16 / L::VROW, place = lane * 16 % L::VROW / 16;
+      voff = d * page * L::ES + (place ^ L::value_turn(d)) * 16;
+      Places first[L::SLOTS];
+#pragma unroll
+      for (int i = 0; i < L::SLOTS; ++i) first[i] = find();
+      next_own = find();
+#pragma unroll
+      for (int i = 0; i < L::SLOTS; ++i)
+        if (i < mine) issue_own(i, first[i]);
+    }
+  } else {
+    find_stage();
+#pragma unroll
+    for (int i = 0; i < L::STAGES - 1; ++i)
+      if (i < count) {
+        issue_stage(i, i);
+        find_stage();
+      }
+  }
 
   // ---- the wave's columns
   int limit[CT];                                            // keys that the lane's column sees end here
@@ -187,7 +242,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
   Frag qf[CT][QS];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int c0 = col0 + (wave * CT + ct) * 16, c = c0 + col;
+    const int c0 = col0 + ((apart ? 0 : wave * CT) + ct) * 16, c = c0 + col;
     const bool ok = c < columns;
     if (c0 < columns) tiles = ct + 1;
     const int r = first_row + (ok ? c / G : 0), head = kvh * G + (ok ? c % G : 0);
@@ -235,6 +290,92 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     return blk + BLOCK_KEYS * h + (HALF ? 8 * kb + j : 16 * (j >> 2) + 4 * kb + (j & 3));
   };
 
+  // a lane's piece s of the keys' rows of score tile t, piece f of the values, of 32 keys in the LDS
+  auto key_frag = [&](const char* at, int t, int s) {
+    const int r = HALF ? 8 * (col >> 2) + 4 * t + (col & 3) : 16 * t + col;
+    const bool beyond = HALF && D % 32 != 0 && s == KS - 1 && kb >= 2;          // the last step of 32 dims is half empty
+    Frag a;
+    a.q = *reinterpret_cast<const uint4*>(at + r * L::ROW + ((beyond ? 0 : 4 * s + kb) ^ L::key_turn(r)) * 16);
+    if (beyond) a.q = make_uint4(0, 0, 0, 0);
+    return a;
+  };
+  auto value_frag = [&](const char* at, int f) {
+    const int d = (HALF ? f : f >> 1) * 16 + col, half = HALF ? kb >> 1 : f & 1, place = HALF ? kb & 1 : kb;
+    Frag a;
+    a.q = *reinterpret_cast<const uint4*>(at + L::TILE + (half * D + d) * L::VROW + (place ^ L::value_turn(d)) * 16);
+    return a;
+  };
+  // 0 * (whatever is in slots that no column sees) must not reach a sum
+  auto clear_hidden = [&](Frag& v, int f, int blk, int h) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (HALF) {
+        const int key = key_at(blk, h, 2 * j);
+        v.w[j] &= (key >= key_begin && key < most ? 0x0000FFFFu : 0u) | (key + 1 >= key_begin && key + 1 < most ? 0xFFFF0000u : 0u);
+      } else {
+        const int key = key_at(blk, h, 4 * (f & 1) + j);
+        if (key < key_begin || key >= most) v.w[j] = 0;
+      }
+    }
+  };
+  // The first tile of columns through 32 keys whose pieces are in registers.
+  auto attend_one = [&](Frag (&a)[2][QS], Frag (&va)[HALF ? DT : 2 * DT], int blk) {
+    f32x4 S[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int s = 0; s < QS; ++s)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (HALF) {
+          S[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][s].v, qf[0][s].v, S[t], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[t][s].w[j]), __uint_as_float(qf[0][s].w[j]), S[t], 0, 0, 0);
+        }
+      }
+    if (blk < key_begin || blk + BLOCK_KEYS > least) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = key_at(blk, 0, j);
+        if (key < key_begin || key >= limit[0]) S[j >> 2][j & 3] = -INFINITY;
+      }
+#pragma unroll
+      for (int f = 0; f < (HALF ? DT : 2 * DT); ++f) clear_hidden(va[f], f, blk, 0);
+    }
+    float mx = S[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, S[j >> 2][j & 3]);
+    mx = quad_max(mx) * scale_log2;
+    if (__any(mx > m[0] + 8.f)) {
+      const float m_new = fmaxf(m[0], mx);
+      const float alpha = m[0] == -INFINITY ? 0.f : fast_exp2(m[0] - m_new);
+      m[0] = m_new;
+      l[0] *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) O[0][dt] *= alpha;
+    }
+    const float base = m[0] == -INFINITY ? 0.f : m[0];
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = fast_exp2(fmaf(S[j >> 2][j & 3], scale_log2, -base));
+      l[0] += p[j];
+    }
+    if constexpr (HALF) {
+      Frag pb;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pb.w[j] = pack_bf16(p[2 * j], p[2 * j + 1]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) O[0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt].v, pb.v, O[0][dt], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          O[0][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va[2 * dt + (j >> 2)].w[j & 3]), p[j], O[0][dt], 0, 0, 0);
+    }
+  };
+
   // NT: the wave's tiles that hold columns, known where this is compiled: with a branch around every product nothing overlaps
   // MASKED: some of the stage's keys are hidden from some columns.
   auto compute = [&](const char* stage, int blk, auto nt, auto masked) {
@@ -246,15 +387,9 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     for (int h = 0; h < L::H; ++h) {
       Frag a[2][QS];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int r = HALF ? 8 * (col >> 2) + 4 * t + (col & 3) : 16 * t + col;
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int s = 0; s < QS; ++s) {
-          const bool beyond = HALF && D % 32 != 0 && s == KS - 1 && kb >= 2;      // the last step of 32 dims is half empty
-          a[t][s].q = *reinterpret_cast<const uint4*>(stage + h * 2 * L::TILE + r * L::ROW + (((beyond ? 0 : 4 * s + kb)) ^ L::key_turn(r)) * 16);
-          if (beyond) a[t][s].q = make_uint4(0, 0, 0, 0);
-        }
-      }
+        for (int s = 0; s < QS; ++s) a[t][s] = key_frag(stage + h * L::SLOT, t, s);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -308,20 +443,10 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
 #pragma unroll
     for (int h = 0; h < L::H; ++h) {
       // the values of 32 keys, asked for before the weights are known
-      const char* vals = stage + h * 2 * L::TILE + L::TILE;
       constexpr int VF = HALF ? DT : 2 * DT;
       Frag va[VF];
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const int d = dt * 16 + col;
-        if constexpr (HALF) {
-          va[dt].q = *reinterpret_cast<const uint4*>(vals + ((kb >> 1) * D + d) * L::VROW + ((kb & 1) ^ L::value_turn(d)) * 16);
-        } else {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            va[2 * dt + t].q = *reinterpret_cast<const uint4*>(vals + (t * D + d) * L::VROW + (kb ^ L::value_turn(d)) * 16);
-        }
-      }
+      for (int f = 0; f < VF; ++f) va[f] = value_frag(stage + h * L::SLOT, f);
       float p[NT][8];
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
@@ -332,20 +457,9 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
           l[ct] += p[ct][j];
         }
       }
-      // 0 * (whatever is in slots that no column sees) must not reach a sum
       if (MASKED && (blk < key_begin || blk + BLOCK_KEYS * (h + 1) > most)) {
 #pragma unroll
-        for (int f = 0; f < VF; ++f)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (HALF) {
-              const int key = key_at(blk, h, 2 * j);
-              va[f].w[j] &= (key >= key_begin && key < most ? 0x0000FFFFu : 0u) | (key + 1 >= key_begin && key + 1 < most ? 0xFFFF0000u : 0u);
-            } else {
-              const int key = key_at(blk, h, 4 * (f & 1) + j);
-              if (key < key_begin || key >= most) va[f].w[j] = 0;
-            }
-          }
+        for (int f = 0; f < VF; ++f) clear_hidden(va[f], f, blk, h);
       }
       if constexpr (HALF) {
         Frag pb[NT];
@@ -396,6 +510,72 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
       if (n < count) step(std::true_type());
     }
   };
+  if constexpr (L::APART) {
+    if (apart) {
+      constexpr int VF = HALF ? DT : 2 * DT;
+      for (int n = 0; n < mine; ++n) {
+        const int blk = blk1 + n * WAVES * BLOCK_KEYS;
+        if (L::SLOTS == 2 && n + 1 < mine) MIE_VMCNT(L::UNITS);        // the wave's next 32 keys may still be on their way
+        else MIE_VMCNT(0);
+        asm volatile("" ::: "memory");
+        const char* slot = lds + (wave * L::SLOTS + (L::SLOTS == 2 ? n & 1 : 0)) * L::SLOT;
+        Frag a[2][QS], va[VF];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int s = 0; s < QS; ++s) a[t][s] = key_frag(slot, t, s);
+#pragma unroll
+        for (int f = 0; f < VF; ++f) va[f] = value_frag(slot, f);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");              // read: the slot is free
+        if (n + L::SLOTS < mine) {
+          issue_own(L::SLOTS == 2 ? n & 1 : 0, next_own);
+          next_own = find();
+        }
+        attend_one(a, va, blk);
+      }
+      // ---- the waves' columns are the same: join them in the LDS, once nobody reads or writes a slot
+      __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+      float* s_o = reinterpret_cast<float*>(lds);
+      const float sum = quad_sum(l[0]);
+      if (kb == 0) {
+        s_m[wave][col] = m[0];
+        s_l[wave][col] = sum;
+      }
+      __syncthreads();
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) M = fmaxf(M, s_m[w][col]);
+      const float f = m[0] == -INFINITY ? 0.f : fast_exp2(m[0] - M);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s_o[(wave * 16 + col) * (D + 1) + dt * 16 + 4 * kb + i] = O[0][dt][i] * f;
+      __syncthreads();
+      for (int e = threadIdx.x; e < 16 * D; e += WAVES * 64) {
+        const int hc = e / D, d = e - hc * D, c = col0 + hc;
+        if (c >= columns) break;
+        float M1 = -INFINITY, total = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) M1 = fmaxf(M1, s_m[w][hc]);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+          total += s_m[w][hc] == -INFINITY ? 0.f : fast_exp2(s_m[w][hc] - M1) * s_l[w][hc];
+          y += s_o[(w * 16 + hc) * (D + 1) + d];
+        }
+        const int r = first_row + c / G, head = kvh * G + c % G;
+        if (row_parts[r + 1] - row_parts[r] == 1) {
+          const float sink = head_sinks ? head_sinks[head] * 1.4426950408889634f : sink_log2;
+          const float all = total + (sink == -INFINITY ? 0.f : M1 == -INFINITY ? 1.f : fast_exp2(sink - M1));
+          out[((size_t)r * Hq + head) * D + d] = from_float<T>(all == 0.f ? 0.f : y / all);
+        } else {
+          const size_t at = (size_t)(row_parts[r] + part) * Hq + head;
+          o_part[at * D + d] = total == 0.f ? 0.f : y / total;
+          if (d == 0) lse_part[at] = total == 0.f ? -INFINITY : M1 + log2f(total);
+        }
+      }
+      return;
+    }
+  }
   if (CT == 2 && tiles == 2) walk(std::integral_constant<int, CT>());
   else if (tiles > 0) walk(std::integral_constant<int, 1>());
   else walk(std::integral_constant<int, 0>());
@@ -506,7 +686,7 @@ static int launch_items(const void* q, long q_stride, const void* k_cache, const
                         const int* row_parts, int Hq, int Hkv, int page, float scale, float sink, const float* head_sinks, hipStream_t stream) {
   auto* kernel = shared_attention_kernel<T, CT>;
   constexpr int lds = Layout<T, CT>::LDS;
-  if (lds > 65536 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, "shared_prefix_attention")) return -1;
+  if (lds > 65536 - 1024 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, "shared_prefix_attention")) return -1;
   const int q_vec = ((uintptr_t)q & 15) == 0 && (q_stride * (long)sizeof(T)) % 16 == 0;
   hipLaunchKernelGGL(kernel, dim3((unsigned)num_items * Hkv), dim3(WAVES * 64), lds, stream, (const T*)q, q_stride, q_vec,
                      (const T*)k_cache, (const T*)v_cache, (T*)out, o_part, lse_part, tables, max_blocks, pages, positions,

@@ -19,7 +19,7 @@ class SharedPrefixPlan:
     most keys each row has while the plan is used (its position + 1, or more: a plan holds for as many steps as its rows and
     shared keys stay and their contexts suffice).  Made once a step, or once for many, and used by every layer of it."""
 
-    def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256, least_keys=64, per_unit=2):
+    def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256, least_keys: int = 64, per_unit: float = 1):
         contexts = [int(c) for c in contexts]
         groups = [(int(n), int(k)) for n, k in groups]
         if num_kv_heads < 1 or num_q_heads % num_kv_heads:
@@ -50,7 +50,7 @@ class SharedPrefixPlan:
         tiles = [-(-w[1] // wide) for w in work]
         total = sum(t * (w[3] - w[2]) for w, t in zip(work, tiles)) * num_kv_heads
         # keys an item: two items a compute unit, and no less than 64 (an item's start and its partial result cost about as much)
-        most = max(least_keys, -(-total // (per_unit * units) // BLOCK_KEYS) * BLOCK_KEYS)
+        most = max(least_keys, -(-total // int(per_unit * units) // BLOCK_KEYS) * BLOCK_KEYS)
         parts = np.zeros(self.num_rows, dtype=np.int64)
         items, several = [], []
         for (row, columns, begin, end), t in zip(work, tiles):
