@@ -472,11 +472,12 @@ class KernelBackend:
         Returns [T, Hq * D] in act_dtype."""
         raise NotImplementedError
 
-    def plan_shared_prefix(self, groups, contexts, num_q_heads, num_kv_heads, head_dim):
+    def plan_shared_prefix(self, groups, contexts, num_q_heads, num_kv_heads, head_dim, share=None):
         """The plan (kernels.shared_prefix.SharedPrefixPlan) of steps of single-token rows whose requests share the first part of
         their cache: ``groups`` = (rows, keys) of every run of rows, in order, ``keys`` the number of first keys that the rows of the
         run share (0: none); ``contexts``: for each row the most keys it has while the plan is used (position + 1, or more).  A
-        plan serves every layer of a step, and later steps as long as rows, shared keys and contexts hold."""
+        plan serves every layer of a step, and later steps as long as rows, shared keys and contexts hold.  ``share``: read shared
+        keys once (True), by every row for itself (False), or whichever is faster (None)."""
         raise NotImplementedError
 
     def shared_prefix_attention(self, qkv, num_q_heads, num_kv_heads, head_dim, k_cache, v_cache, group, step, scale, plan, sink=None):

@@ -100,6 +100,7 @@ class HipBackend(KernelBackend):
         if not torch.cuda.is_available():
             raise RuntimeError("no GPU visible to torch: the engine needs an MI355X (gfx950)")
         self._libs = {}
+        self._units = None          # compute units
         self._shared_libs = {}      # of attention over shared keys, by head size
         self._rule_slices = {}      # slices that choosing under rules cuts a row into, by rows and vocabulary
         self._zeros = None          # 256 zero bytes on the device, what masked loads of grouped products read
@@ -1995,9 +1996,10 @@ class HipBackend(KernelBackend):
         return True
 
     # ---- rows that share the first part of their cache (csrc/shared_attention.hip)
-    def plan_shared_prefix(self, groups, contexts, num_q_heads, num_kv_heads, head_dim):
-        return SharedPrefixPlan(groups, contexts, num_q_heads, num_kv_heads, head_dim, self.device,
-                                torch.cuda.get_device_properties(self._device_index).multi_processor_count)
+    def plan_shared_prefix(self, groups, contexts, num_q_heads, num_kv_heads, head_dim, share=None):
+        if self._units is None:
+            self._units = torch.cuda.get_device_properties(self._device_index).multi_processor_count
+        return SharedPrefixPlan(groups, contexts, num_q_heads, num_kv_heads, head_dim, self.device, self._units, self.true_fp32, share)
 
     def shared_prefix_attention(self, qkv, num_q_heads, num_kv_heads, head_dim, k_cache, v_cache, group, step, scale, plan, sink=None):
         Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim

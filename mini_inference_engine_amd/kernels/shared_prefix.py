@@ -2,8 +2,8 @@
 
 A step of single-token rows falls into runs of rows; the rows of a run share their first ``keys`` keys, read through the block
 table of the run's first row.  The plan cuts the step into items, each one workgroup a kv head (csrc/shared_attention.hip):
-columns (query heads of rows) x keys, so that all items take about the same time and there are enough of them for
-the GPU.  An item leaves a partial result for each of its columns; a row's partial results are its items in order of keys.
+columns (query heads of rows) x keys, so that all items take about the same time and there are as many as compute units.
+An item leaves a partial result for each of its columns; a row's partial results are its items in order of keys.
 """
 from __future__ import annotations
 
@@ -12,56 +12,70 @@ import torch
 
 TILE = 64               # columns that a workgroup's four waves take with one tile of 16 each
 BLOCK_KEYS = 32
+LEAST_KEYS = 64         # of a cut: an item's start and its partial result cost about as much
 
 
 class SharedPrefixPlan:
     """Who shares what in a step of single-token rows.  ``groups``: (rows, keys) of every run of rows, in order; ``contexts``: the
     most keys each row has while the plan is used (its position + 1, or more: a plan holds for as many steps as its rows and
-    shared keys stay and their contexts suffice).  Made once a step, or once for many, and used by every layer of it."""
+    shared keys stay and their contexts suffice).  Made once a step, or once for many, and used by every layer of it; on another
+    stream than the one it was made on only once that has been waited for.  ``share``: whether shared keys are read once for all
+    (True), by every row for itself (False), or what is faster (None)."""
 
-    def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256, least_keys: int = 64, per_unit: float = 1):
+    def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256,
+                 float32: bool = False, share: bool | None = None):
         contexts = [int(c) for c in contexts]
         groups = [(int(n), int(k)) for n, k in groups]
-        if num_kv_heads < 1 or num_q_heads % num_kv_heads:
+        if num_kv_heads < 1 or num_q_heads < 1 or num_q_heads % num_kv_heads:
             raise ValueError(f"shared prefix: {num_q_heads} query heads are not a multiple of {num_kv_heads} kv heads")
         if any(n < 1 or k < 0 for n, k in groups) or sum(n for n, _ in groups) != len(contexts):
             raise ValueError(f"shared prefix: runs of rows {groups[:8]} for {len(contexts)} rows")
         if any(c < 0 or c > 0x7FFFFF00 for c in contexts):
             raise ValueError("shared prefix: contexts are numbers of keys, 0 or more")
+        first = 0
+        for n, k in groups:
+            if any(c < k for c in contexts[first:first + n]):
+                raise ValueError(f"shared prefix: rows {first} to {first + n - 1} share {k} keys, and one of them has fewer")
+            first += n
         self.num_rows, self.num_q_heads, self.num_kv_heads, self.head_dim = len(contexts), int(num_q_heads), int(num_kv_heads), int(head_dim)
         self.contexts = np.asarray(contexts, dtype=np.int64)
         self.max_context = max(contexts, default=0)
         G = num_q_heads // num_kv_heads
-        first, work = 0, []                         # (first row, columns, first key, keys) of what is to be cut
+        whole = not self._worth_it(G, units, float32) if share is None else not share
+        if whole:
+            groups = [(1, 0)] * self.num_rows
+
+        first, work = 0, []                         # (first row, columns, first key, end) of what is to be cut
         for n, k in groups:
-            if any(c < k for c in contexts[first:first + n]):
-                raise ValueError(f"shared prefix: rows {first} to {first + n - 1} share {k} keys, and one of them has fewer")
-            if n == 1:
-                k = 0                               # nobody to share with
-            elif k:
+            k = 0 if n == 1 else k                  # a single row has nobody to share with
+            if k:
                 work.append((first, n * G, 0, k))
-            for r in range(first, first + n):
-                if contexts[r] > k:
-                    work.append((r, G, k, contexts[r]))
+            work += [(r, G, k, contexts[r]) for r in range(first, first + n) if contexts[r] > k]
             first += n
         widest = max((w[1] for w in work), default=1)
         self.column_tiles = 2 if widest > TILE and head_dim <= 128 else 1
         wide = TILE * self.column_tiles
         tiles = [-(-w[1] // wide) for w in work]
-        total = sum(t * (w[3] - w[2]) for w, t in zip(work, tiles)) * num_kv_heads
-        # keys an item: two items a compute unit, and no less than 64 (an item's start and its partial result cost about as much)
-        most = max(least_keys, -(-total // int(per_unit * units) // BLOCK_KEYS) * BLOCK_KEYS)
+        # What a key of an item costs, in keys of an item of up to 16 columns, whose waves share out the keys: measured, us for 64 keys in
+        # bfloat16 0.4, of up to 64 columns 0.9, of 128 columns 1.3 (head size 128); the 32-bit products of float32 weigh more.
+        wider = (4, 8) if float32 else (2, 3)
+        cost = [1 if w[1] <= 16 else wider[min(w[1], wide) > TILE] for w in work]
+        total = sum(t * c * (w[3] - w[2]) for w, t, c in zip(work, tiles, cost)) * num_kv_heads
+        # One compute unit's share.  Items of half of it balance better and leave twice the partial results: over fifteen shapes in
+        # geometric mean 35.3 us, 33.2 at two thirds, 31.9 at this, 33.9 at four thirds.
+        most = -(-total // units)
+
         parts = np.zeros(self.num_rows, dtype=np.int64)
         items, several = [], []
-        for (row, columns, begin, end), t in zip(work, tiles):
-            pieces = -(-(end - begin) // most)
+        for (row, columns, begin, end), t, c in zip(work, tiles, cost):
+            pieces = 1 if whole and share is None else -(-(end - begin) // max(LEAST_KEYS, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
             size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
             rows = columns // G
             at = begin
             while at < end:
                 # cuts lie on whole blocks of the cache, so that no block is read twice
                 to = end if end - at <= size else (at + size) // BLOCK_KEYS * BLOCK_KEYS
-                (several if rows > 1 else items).extend((row, columns, c * wide, at, to, int(parts[row]), 0, 0) for c in range(t))
+                (several if rows > 1 else items).extend((row, columns, i * wide, at, to, int(parts[row]), 0, 0) for i in range(t))
                 parts[row:row + rows] += 1
                 at = to
         # the longest first: items of many columns take several times what those of one row do (256 rows behind 8,192 keys: the two kinds
@@ -77,6 +91,18 @@ class SharedPrefixPlan:
         data = torch.from_numpy(packed)
         if torch.device(device).type == "cuda":
             data = data.pin_memory().to(device, non_blocking=True)
-        self._data = data
         self.items, self.row_parts = data[:8 * len(items)], data[8 * len(items):]
         self.addresses = self.items.data_ptr(), self.row_parts.data_ptr()
+
+    def _worth_it(self, G: int, units: int, float32: bool) -> bool:
+        """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup a kv head, with no partial
+        results and no second launch: as long as that takes no longer than the second launch costs.  Measured, us a call one after another,
+        whole / shared (4 heads of 64 and 8 of 128, 4 to 64 rows): 500 keys 11.8 / 16.5, 1,000 keys 11.7 / 16.5 and 11.7 to 16.8 / 16.4 to 19.1;
+        256 rows of 500 keys of 8 heads of 128 58 / 35; float32 500 keys 13 / 16.5 and 21 to 41 / 16.5 to 34, 200 keys 11.6 / 16.5 and 12 to 24 / 16.5
+        to 28."""
+        D, rounds = self.head_dim, -(-self.num_rows * self.num_kv_heads // (2 * units))
+        if G > 16 or D % 32 or D * (4 if float32 else 2) > 512:
+            most = 128                              # one wave computes: see csrc/shared_attention.hip
+        else:
+            most = min(512, 32768 // D) if float32 else min(1024, 131072 // D)
+        return self.max_context * rounds > most

@@ -112,11 +112,14 @@ def ops():
 
 
 def run(ops, s, groups, Hq, Hkv, D, dtype, scale=None, sink=None, contexts=None, **kw):
+    """Shared, not shared, and as the plan chooses by itself."""
     scale = D ** -0.5 if scale is None else scale
     step, group = step_of(s, **kw)
-    plan = ops[dtype].plan_shared_prefix(groups, [p + 1 for p in s.positions.tolist()] if contexts is None else contexts, Hq, Hkv, D)
-    out = ops[dtype].shared_prefix_attention(s.q, Hq, Hkv, D, s.k, s.v, group, step, scale, plan, sink=sink)
-    check(out, *plain(s, Hq, Hkv, D, scale, sink), D, dtype)
+    want = plain(s, Hq, Hkv, D, scale, sink)
+    for share in (True, False, None):
+        plan = ops[dtype].plan_shared_prefix(groups, [p + 1 for p in s.positions.tolist()] if contexts is None else contexts, Hq, Hkv, D, share=share)
+        out = ops[dtype].shared_prefix_attention(s.q, Hq, Hkv, D, s.k, s.v, group, step, scale, plan, sink=sink)
+        check(out, *want, D, dtype)
     return out, plan
 
 
@@ -241,7 +244,7 @@ def test_in_a_graph_and_on_another_stream(ops):
     groups = [(12, 700), (4, 0)]
     s = make(groups, [720 + i for i in range(12)] + [5, 90, 300, 719], 8, 2, 64, 16, BF16, poison=False)
     step, group = step_of(s, host={})
-    plan = ops[BF16].plan_shared_prefix(groups, [p + 1 for p in s.positions.tolist()], 8, 2, 64)
+    plan = ops[BF16].plan_shared_prefix(groups, [p + 1 for p in s.positions.tolist()], 8, 2, 64, share=True)
     call = lambda: ops[BF16].shared_prefix_attention(s.q, 8, 2, 64, s.k, s.v, group, step, 0.125, plan)     # noqa: E731
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -274,9 +277,10 @@ def test_pages_beyond_32_bits_of_offset(ops, dtype):
     k[pages - small.k.shape[0]:] = small.k
     v[pages - small.k.shape[0]:] = small.v
     step, _ = step_of(small)
-    plan = ops[dtype].plan_shared_prefix([(3, 40)], [46, 51, 40], Hq, Hkv, D)
-    out = ops[dtype].shared_prefix_attention(small.q, Hq, Hkv, D, k, v, SimpleNamespace(block_tables=far.contiguous()), step, 0.1, plan)
-    check(out, *plain(small, Hq, Hkv, D, 0.1), D, dtype)
+    for share in (True, False):
+        plan = ops[dtype].plan_shared_prefix([(3, 40)], [46, 51, 40], Hq, Hkv, D, share=share)
+        out = ops[dtype].shared_prefix_attention(small.q, Hq, Hkv, D, k, v, SimpleNamespace(block_tables=far.contiguous()), step, 0.1, plan)
+        check(out, *plain(small, Hq, Hkv, D, 0.1), D, dtype)
 
 
 # ---- the plan, on the CPU
@@ -312,14 +316,18 @@ def covered(plan, groups, contexts, G):
         first += n
 
 
+@pytest.mark.parametrize("share", [True, False, None])
 @pytest.mark.parametrize("seed", range(40))
-def test_a_plan_covers_every_key_once(seed):
+def test_a_plan_covers_every_key_once(seed, share):
     g = np.random.RandomState(seed)
     groups = [(int(g.randint(1, 40)), int(g.choice([0, 1, 31, 32, 500, 7000, 40000]))) for _ in range(g.randint(1, 6))]
     contexts = [k + int(g.choice([0, 1, 2, 33, 900])) for n, k in groups for _ in range(n)]
     G, Hkv = int(g.choice([1, 3, 8, 16])), int(g.choice([1, 4, 8]))
-    plan = SharedPrefixPlan(groups, contexts, G * Hkv, Hkv, 64, "cpu")
+    plan = SharedPrefixPlan(groups, contexts, G * Hkv, Hkv, 64, "cpu", float32=bool(seed % 2), share=share)
     covered(plan, groups, contexts, G)
+    shared = any(columns > G for _, columns, *_ in plan.items.view(-1, 8).tolist())
+    if share is not None:
+        assert shared == (share and any(n > 1 and k > 0 for n, k in groups))
 
 
 @pytest.mark.parametrize("bad", [([(2, 5)], [5, 4], 4, 2), ([(2, 5)], [5], 4, 2), ([(0, 5), (1, 0)], [5], 4, 2), ([(1, -1)], [5], 4, 2),
