@@ -73,7 +73,9 @@ def cmd_generate(args) -> int:
     else:
         print("give --prompt-ids, --prompt-lens or --prompt", file=sys.stderr)
         return 2
-    sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, ignore_eos=args.ignore_eos)
+    sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, ignore_eos=args.ignore_eos,
+                        repetition_penalty=args.repetition_penalty, presence_penalty=args.presence_penalty,
+                        frequency_penalty=args.frequency_penalty)
     outs = eng.generate(prompts, sp)
     for o in outs:
         print(json.dumps({"seq_id": o.seq_id, "prompt_len": o.prompt_len, "output_ids": o.output_ids, "text": o.text,
@@ -109,6 +111,9 @@ def main(argv=None) -> int:
     g.add_argument("--max-tokens", type=int, default=128)
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--ignore-eos", action="store_true")
+    g.add_argument("--repetition-penalty", type=float, default=1.0)
+    g.add_argument("--presence-penalty", type=float, default=0.0)
+    g.add_argument("--frequency-penalty", type=float, default=0.0)
     g.add_argument("--max-num-batched-tokens", dest="max_num_batched_tokens", type=int)
     g.add_argument("--max-num-seqs", dest="max_num_seqs", type=int)
     g.add_argument("--num-blocks", dest="num_blocks", type=int)

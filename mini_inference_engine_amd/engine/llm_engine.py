@@ -16,7 +16,7 @@ from dataclasses import dataclass, replace
 import torch
 
 from ..config.engine_config import EngineConfig
-from ..sampling import Sampler, SamplingParams
+from ..sampling import RuleInputs, Sampler, SamplingParams
 from .batch import StepRow
 from .runner import ModelRunner, parse_dtype
 from .scheduler import Scheduler
@@ -67,7 +67,9 @@ class LLMEngine:
         if cfg.trace_ranges and self.runner.device.type == "cuda":
             self.runner.ranges.on = True
         self._in_flight = None             # the step whose tokens the host has not read yet
+        self._reading = set()              # live requests that look at their output before each token (allowed_tokens)
         self.stop_token_ids = frozenset(self.runner.model.spec.stop_token_ids)
+        self.rule_inputs = RuleInputs(self.runner.device, self.runner.vocab_size)
         if verbose:
             print(f"[mini_inference_engine_amd] cache: {self.runner.num_pages} pages x {cfg.block_size} tokens "
                   f"({self.runner.storage.num_bytes() / 2**30:.2f} GiB), weights "
@@ -110,6 +112,9 @@ class LLMEngine:
         bad = [t for t in ids if not 0 <= t < vocab]
         if bad:
             raise ValueError(f"token ids outside the vocabulary of {vocab}: {bad[:5]}")
+        bad = [t for t in params.logit_bias or () if not 0 <= t < vocab]
+        if bad:
+            raise ValueError(f"logit_bias for tokens outside the vocabulary of {vocab}: {bad[:5]}")
         if len(ids) + params.max_tokens > self.cfg.max_model_len:
             params = replace(params, max_tokens=self.cfg.max_model_len - len(ids))
         seq = Sequence(ids, params)
@@ -117,6 +122,10 @@ class LLMEngine:
             seq.seed = (self.cfg.seed << 32) ^ self._num_requests
         self._num_requests += 1
         self.scheduler.add(seq)
+        if params.has_penalties:
+            self.runner.keep_token_history()
+        if params.allowed_tokens is not None:
+            self._reading.add(seq)
         return seq
 
     # ------------------------------------------------------------------- step
@@ -131,9 +140,16 @@ class LLMEngine:
         Running one step ahead: a request's next row is scheduled before its last token is known to the
         host; the device takes the token from where the sampling kernel left it.  What does not depend on
         the token's value (positions, pages, the end by max_tokens or length) is decided at once; an end
-        by the stop token is seen one step late, and the row already started for that request is dropped."""
+        by the stop token is seen one step late, and the row already started for that request is dropped.
+        While a request with ``allowed_tokens`` is there, whose next token depends on the value of its last, nothing
+        runs ahead."""
+        ahead = self.cfg.run_ahead and not self._reading
+        if not ahead and self._in_flight is not None:
+            finished = self.drain()
+            if finished:
+                return finished
         started = self._start()
-        if not self.cfg.run_ahead:
+        if not ahead:
             return self._finish_step(started) if started is not None else []
         finished = self._finish_step(self._in_flight) if self._in_flight is not None else []
         self._in_flight = started
@@ -169,7 +185,13 @@ class LLMEngine:
                 sample_seqs.append(seq)
 
         # a captured graph when every row is a single token; the tokens are chosen in the step as well
-        self.runner.forward_step(rows, sampling=self.sampler.sampling_inputs(sample_seqs) if sample_seqs else None)
+        sampling = rules = None
+        if sample_seqs:
+            sampling = self.sampler.sampling_inputs(sample_seqs)
+            if any(s.params.has_rules for s in sample_seqs):
+                self.rule_inputs.stop_token_ids = sorted(self.stop_token_ids)
+                rules = self.rule_inputs.make(sample_seqs, [s.num_tokens for s in sample_seqs], self.runner.token_history)
+        self.runner.forward_step(rows, sampling=sampling, **({} if rules is None else {"rules": rules}))
         self.num_steps += 1
         self.num_graph_steps += self.runner.last_step_captured
         chosen = self.sampler.fetch_async(len(sample_seqs)) if sample_seqs else None
@@ -199,6 +221,7 @@ class LLMEngine:
             if not (stopped or (seq.ending and place == seq.num_tokens - 1)):
                 continue
             del seq.token_ids[place + 1:]      # a placeholder of the row started meanwhile, if any
+            self._reading.discard(seq)
             seq.finish_time = now
             if seq.status is Status.RUNNING:
                 self.scheduler.finish(seq)

@@ -106,6 +106,7 @@ class ModelRunner:
         # The tokens the last step chose, at a fixed address: the next step's rows may take their token
         # from here on the device (StepRow.taken_from) before the host has seen it.
         self.chosen_tokens = torch.zeros(max(1, max_rows), dtype=torch.int32, device=self.device)
+        self.token_history = None           # [slots, positions] int32: every request's tokens (keep_token_history)
         self.graphs = None                  # captured decode steps, once capture_decode_graphs was called
         self.portion_graphs = []            # captured steps of one prompt portion, by token count (capture_portion_graphs)
         self.last_step_captured = False
@@ -122,7 +123,17 @@ class ModelRunner:
         with self.ranges("prepare"):
             step = build_step(rows, self.arena, self.page_size, **kw)
         step.earlier_tokens = self.chosen_tokens
+        if self.token_history is not None:
+            self.ops.record_tokens(self.token_history, step)
         return step
+
+    def keep_token_history(self) -> torch.Tensor:
+        """From now on every step's tokens are also written to ``token_history`` [state slots, positions]: a request's text where the
+        rules on its logits look for it (kernels.api.LogitRules).  A request has its whole text there if its first step comes later."""
+        if self.token_history is None:
+            positions = min(self.max_model_len, self.cache.max_tokens_one_request())
+            self.token_history = torch.zeros((self.num_state_slots, positions), dtype=torch.int32, device=self.device)
+        return self.token_history
 
     def capture_decode_graphs(self, batch_sizes, verbose: bool = False, sample: bool = False) -> None:
         """Capture the forward of a step of single-token rows once per batch size; ``forward_step``
@@ -161,14 +172,17 @@ class ModelRunner:
         return None
 
     @torch.inference_mode()
-    def forward_step(self, rows: list[StepRow], sampling=None) -> torch.Tensor | None:
+    def forward_step(self, rows: list[StepRow], sampling=None, rules=None) -> torch.Tensor | None:
         """Logits [sum of wants, vocab] float32, ordered by row then by ``want``.
         Pages for the rows' tokens must have been reserved.
 
         ``sampling``: (temperatures, seeds, counters), one entry for each wanted row of logits: the step also
         chooses a token from each of them on the device (temperature 0: the largest logit; else a draw whose
         noise is a function of seed and counter) and leaves it in ``chosen_tokens[i]``.  The three arrays
-        travel with the step's other arrays, and in a captured step the choice is part of the graph."""
+        travel with the step's other arrays, and in a captured step the choice is part of the graph.
+
+        ``rules`` (LogitRules of the wanted rows, beside ``sampling``): the tokens are chosen under them, from logits
+        that are returned as they are."""
         self.last_step_captured = False
         captured = (self.graphs is not None and self.graphs.fits(len(rows)) and all(len(r.tokens) == 1 for r in rows)
                     and (sampling is None or all(len(r.want) == 1 for r in rows)))
@@ -179,7 +193,7 @@ class ModelRunner:
         elif captured:
             self.last_step_captured = True
             logits, step = self.graphs.run(self, rows, sampling)
-            if sampling is None or self.graphs.sample:
+            if sampling is None or (self.graphs.sample and rules is None):
                 return logits
         else:
             step = self.build(rows, sampling=sampling)
@@ -188,8 +202,9 @@ class ModelRunner:
         if sampling is not None and logits is not None:
             n = logits.shape[0]
             with self.ranges("sample"):
+                under = {} if rules is None else {"rules": rules}        # (a backend that knows none is not handed any)
                 self.ops.sample(logits, step.sample_temps[:n], step.sample_seeds[:n], step.sample_counters[:n],
-                                out=self.chosen_tokens[:n])
+                                out=self.chosen_tokens[:n], **under)
         return logits
 
     def after_step(self, rows: list[StepRow]) -> None:

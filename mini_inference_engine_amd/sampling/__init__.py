@@ -1,2 +1,3 @@
 from .params import SamplingParams
+from .rules import RuleInputs
 from .sampler import Sampler
