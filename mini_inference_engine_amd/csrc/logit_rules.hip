@@ -66,7 +66,7 @@ __device__ __forceinline__ float apply_rules(float z, uint32_t w, const RowRules
 // Grid (workgroups a row, rows); a workgroup takes every gridDim.x-th slice.  CHOOSE: its best candidate to best_v, best_i [rows,
 // workgroups], or, of a row that has one workgroup, the token to ``chosen``; else the adjusted logits to ``out``.
 template <bool CHOOSE, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == PART_THREADS ? (CHOOSE ? 8 : 5) : 4)
 rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float* out, long out_ld,
              const float* __restrict__ temperatures, const long long* __restrict__ seeds, const int* __restrict__ counters,
              float* __restrict__ best_v, int* __restrict__ best_i, int* __restrict__ chosen) {
@@ -147,7 +147,7 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
         }
       };
       const int length4 = length & ~3;
-      constexpr int READS = 4;                                        // on their way together
+      constexpr int READS = CHOOSE ? 2 : 4;                           // on their way together
       for (int i0 = tid * 4; i0 < length4; i0 += READS * THREADS * 4) {
         i32x4_any t[READS];
 #pragma unroll
@@ -177,15 +177,15 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
       if (i >= n4) break;
       uint4 w = make_uint4(0, 0, 0, 0);
       if (counted) w = *reinterpret_cast<const uint4*>(words + i);
-      f32x4_any y;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t wj = j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
-        y[j] = bits[k] >> j & 1 ? apply_rules(z[k][j], wj, row) : -INFINITY;
-        if (wj & BIASED) y[j] = z[k][j];                              // left to the list, below
-        else if (CHOOSE) sample_consider(y[j], begin + i + j, noisy, inv_t, key, bv, bi);
+        const float y = bits[k] >> j & 1 ? apply_rules(z[k][j], wj, row) : -INFINITY;
+        if (wj & BIASED) continue;                                    // left as it is to the list, below
+        if (CHOOSE) sample_consider(y, begin + i + j, noisy, inv_t, key, bv, bi);
+        else z[k][j] = y;
       }
-      if (!CHOOSE) *reinterpret_cast<f32x4_any*>(o0 + i) = y;
+      if (!CHOOSE) *reinterpret_cast<f32x4_any*>(o0 + i) = z[k];
     }
     if (n4 + tid < n) {                                               // up to three at the end of the row
       const int i = n4 + tid;
