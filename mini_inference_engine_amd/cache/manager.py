@@ -11,7 +11,8 @@ optional watermark; everything a request holds goes back when it ends or is
 preempted.  Beyond the reference: a windowed group also gives back pages that
 lie wholly before the window once a step has passed them (their table entries
 become 0, the scratch page), except those of a request's first tokens that the
-group keeps, and every request holds a state slot.
+group keeps, every request holds a state slot, and a request may begin with pages
+another one has filled (``fork``).
 """
 from __future__ import annotations
 
@@ -77,8 +78,26 @@ class CacheManager:
         rc.closed = True
         del self.live[rc.request_id]
 
+    def fork(self, rc: RequestCache, request_id, tokens: int) -> RequestCache:
+        """A request whose first ``tokens`` tokens are those of ``rc``, which has them in the cache: it opens holding the pages that are
+        full of them (tokens // page_size; nobody writes to a full page) and runs its tokens from there on.  Not where a
+        group gives pages back as its window moves on, nor for a model with state of fixed size, which would have to be as it was
+        after those tokens."""
+        if rc.closed:
+            raise CacheAccountingError(f"request {rc.request_id!r} is closed")
+        if self.on_open is not None or any(g.window is not None for g in self.groups):
+            raise CacheAccountingError("requests of a model with windows or state of fixed size cannot be forked")
+        full = tokens // self.page_size
+        if tokens < 0 or any(len(t) < full for t in rc.tables):
+            raise CacheAccountingError(f"request {rc.request_id!r} does not hold {tokens} tokens")
+        new = self.open(request_id)
+        for g, table in enumerate(rc.tables):
+            self.pools[g].share(table[:full])
+            new.tables[g] = list(table[:full])
+        return new
+
     def _release(self, g: int, pages: list[int]) -> None:
-        self.pools[g].give_back(pages)
+        pages = self.pools[g].give_back(pages)
         if self.keep_log:
             self.released_log.extend((g, p) for p in pages)
         if self.on_release is not None and pages:
@@ -146,16 +165,19 @@ class CacheManager:
         return min(full) * self.page_size if full else 1 << 62
 
     def check(self) -> None:
-        """Invariants: every page is free, scratch, or in exactly one table."""
+        """Invariants: every page is free, scratch, or in as many tables as it has holders, once in each."""
         for g, pool in enumerate(self.pools):
             seen = {}
             for rc in self.live.values():
                 for p in rc.tables[g]:
                     if p == 0:
                         continue
-                    if p in seen:
-                        raise CacheAccountingError(f"group {g}: page {p} held by {seen[p]!r} and {rc.request_id!r}")
-                    seen[p] = rc.request_id
+                    if rc.request_id in seen.setdefault(p, []):
+                        raise CacheAccountingError(f"group {g}: page {p} held by {rc.request_id!r} twice")
+                    seen[p].append(rc.request_id)
+            for p, who in seen.items():
+                if len(who) != pool.holders(p):
+                    raise CacheAccountingError(f"group {g}: page {p} held by {who!r}, {pool.holders(p)} holders counted")
             free = list(pool.free)
             if len(set(free)) != len(free):
                 raise CacheAccountingError(f"group {g}: a page is on the free list twice")

@@ -62,8 +62,17 @@ class StepContext:
     max_row_tokens: int = 0          # longest row (host)
     max_context: int = 0             # largest row_context (host), or a static bound when captured
     host: dict = field(default_factory=dict)   # the same arrays as numpy, for parts that plan on the host
+    shared_prefix: list | None = None   # (rows, keys) of runs of rows that share their first keys (ModelRunner.forward_step)
+    prefix_plans: dict = field(default_factory=dict)   # of that, by heads
     shared: dict = field(default_factory=dict)  # what one layer of the step leaves for later ones, by name (tensors over the
                                                 # step's tokens; a layer that gives writes it anew in every forward)
+
+    def prefix_plan(self, ops, num_q_heads: int, num_kv_heads: int, head_dim: int):
+        """The backend's plan of ``shared_prefix`` for layers with such heads, made by the first of them."""
+        key = (num_q_heads, num_kv_heads, head_dim)
+        if key not in self.prefix_plans:
+            self.prefix_plans[key] = ops.plan_shared_prefix(self.shared_prefix, self.host["row_context"], *key)
+        return self.prefix_plans[key]
 
 
 class StepArena:

@@ -135,6 +135,14 @@ class ModelRunner:
             self.token_history = torch.zeros((self.num_state_slots, positions), dtype=torch.int32, device=self.device)
         return self.token_history
 
+    def fork(self, rc, request_id, tokens: int):
+        """CacheManager.fork, with the text of the shared pages where the rules on logits look for it."""
+        new = self.cache.fork(rc, request_id, tokens)
+        if self.token_history is not None:
+            shared = tokens // self.page_size * self.page_size
+            self.token_history[new.state_slot, :shared] = self.token_history[rc.state_slot, :shared]
+        return new
+
     def capture_decode_graphs(self, batch_sizes, verbose: bool = False, sample: bool = False) -> None:
         """Capture the forward of a step of single-token rows once per batch size; ``forward_step``
         then replays the smallest captured size that holds such a step instead of launching kernel by
@@ -172,7 +180,7 @@ class ModelRunner:
         return None
 
     @torch.inference_mode()
-    def forward_step(self, rows: list[StepRow], sampling=None, rules=None) -> torch.Tensor | None:
+    def forward_step(self, rows: list[StepRow], sampling=None, rules=None, shared_prefix=None) -> torch.Tensor | None:
         """Logits [sum of wants, vocab] float32, ordered by row then by ``want``.
         Pages for the rows' tokens must have been reserved.
 
@@ -182,11 +190,17 @@ class ModelRunner:
         travel with the step's other arrays, and in a captured step the choice is part of the graph.
 
         ``rules`` (LogitRules of the wanted rows, beside ``sampling``): the tokens are chosen under them, from logits
-        that are returned as they are."""
+        that are returned as they are.
+
+        ``shared_prefix``: (rows, keys) of runs of rows, in order, that hold the same pages for their first ``keys``
+        tokens (CacheManager.fork; whole pages, 0: nothing shared), for a step of single-token rows: layers that see all
+        earlier keys then read the shared ones once a run (KernelBackend.shared_prefix_attention).  Such a step is not a captured one."""
+        if shared_prefix is not None:
+            self._check_shared_prefix(rows, shared_prefix)
         self.last_step_captured = False
-        captured = (self.graphs is not None and self.graphs.fits(len(rows)) and all(len(r.tokens) == 1 for r in rows)
+        captured = (shared_prefix is None and self.graphs is not None and self.graphs.fits(len(rows)) and all(len(r.tokens) == 1 for r in rows)
                     and (sampling is None or all(len(r.want) == 1 for r in rows)))
-        portion = None if captured or not self.portion_graphs else self._portion_graph_for(rows)
+        portion = None if captured or shared_prefix is not None or not self.portion_graphs else self._portion_graph_for(rows)
         if portion is not None:
             self.last_step_captured = True
             logits, step = portion.run(self, rows, sampling)
@@ -197,6 +211,7 @@ class ModelRunner:
                 return logits
         else:
             step = self.build(rows, sampling=sampling)
+            step.shared_prefix = shared_prefix
             with self.ranges("forward"):
                 logits = self.model.forward(step)
         if sampling is not None and logits is not None:
@@ -206,6 +221,20 @@ class ModelRunner:
                 self.ops.sample(logits, step.sample_temps[:n], step.sample_seeds[:n], step.sample_counters[:n],
                                 out=self.chosen_tokens[:n], **under)
         return logits
+
+    def _check_shared_prefix(self, rows, runs) -> None:
+        if any(len(r.tokens) != 1 for r in rows) or sum(n for n, _ in runs) != len(rows) or any(n < 1 for n, _ in runs):
+            raise ValueError(f"shared first parts of {sum(n for n, _ in runs)} rows for a step of {len(rows)}, all of single tokens")
+        first = 0
+        for n, keys in runs:
+            run = rows[first:first + n]
+            if keys < 0 or keys % self.page_size or any(r.start < keys for r in run):
+                raise ValueError(f"rows {first} to {first + n - 1} share {keys} keys: whole pages of {self.page_size}, before each row's token")
+            for g, group in enumerate(self.cache.groups):
+                pages = run[0].cache.tables[g][:keys // self.page_size]
+                if group.window is None and any(r.cache.tables[g][:len(pages)] != pages for r in run[1:]):
+                    raise ValueError(f"rows {first} to {first + n - 1} do not hold the same pages for their first {keys} keys")
+            first += n
 
     def after_step(self, rows: list[StepRow]) -> None:
         """Tell the cache how far each row's request has come (windows release pages)."""

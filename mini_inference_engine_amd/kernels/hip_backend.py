@@ -2003,6 +2003,8 @@ class HipBackend(KernelBackend):
 
     def shared_prefix_attention(self, qkv, num_q_heads, num_kv_heads, head_dim, k_cache, v_cache, group, step, scale, plan, sink=None):
         Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim
+        if isinstance(qkv, ProjectionSums):
+            qkv = qkv.finish()
         T, page, bt = self._check_shared(qkv, Hq, Hkv, D, k_cache, v_cache, group, step, scale, plan)
         dev = self._device_index
         for t in (qkv, k_cache, v_cache, bt, step.positions, plan.items):

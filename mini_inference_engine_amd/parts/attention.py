@@ -3,7 +3,8 @@
 qkv = x W_qkv^T, split [Hq D, Hkv D, Hkv D]; q, k position-encoded; k, v written
 to the cache before attention; query head i reads kv head i // (Hq / Hkv); a
 query at position p sees keys max(0, p - window + 1) .. p of its own request;
-scores * scale, softmax in 32-bit, times V; then the output projection
+scores * scale, softmax in 32-bit, times V (in a step whose rows share the first
+part of their cache, those keys read once for all of them); then the output projection
 (inference_engine/model.py:122-159,172-178).  ``window`` None = all keys (the
 reference has no window).  With ``has_kv`` False the part projects only q and
 must be given another call's cache to read.
@@ -61,6 +62,10 @@ class Attention(Mixer):
         k_cache, v_cache, slots = (cache.k, cache.v, group.slot_mapping) if self.has_kv else (None, None, None)
         qkv = self.position.project_encode_store(ops, x, self.w_qkv, step, self.num_heads, kv_heads_in_row,
                                                  k_cache, v_cache, slots)
-        out = ops.paged_attention(qkv, self.num_heads, self.num_kv_heads, self.head_dim, cache.k, cache.v,
-                                  group, step, self.scale, self.window)
+        if step.shared_prefix is not None and self.window is None and self.scale > 0:
+            out = ops.shared_prefix_attention(qkv, self.num_heads, self.num_kv_heads, self.head_dim, cache.k, cache.v, group, step, self.scale,
+                                              step.prefix_plan(ops, self.num_heads, self.num_kv_heads, self.head_dim))
+        else:
+            out = ops.paged_attention(qkv, self.num_heads, self.num_kv_heads, self.head_dim, cache.k, cache.v,
+                                      group, step, self.scale, self.window)
         return ops.linear(out, self.w_o, add_to=add_to)

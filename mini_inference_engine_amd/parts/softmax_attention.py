@@ -255,6 +255,9 @@ class SoftmaxAttention(Mixer):
             more["keep_first"] = self.keep_first
         if self.chunk is not None:
             more["chunk"] = self.chunk
+        if step.shared_prefix is not None and self.window is None and not more and P <= 256 and self.scale > 0:
+            return ops.shared_prefix_attention(q, H, G, P, cache.k, cache.v, group, step, self.scale, step.prefix_plan(ops, H, G, P),
+                                               sink=self.sink)
         return ops.paged_attention(q, H, G, P, cache.k, cache.v, group, step, self.scale, self.window, sink=self.sink, **more)
 
     @property
