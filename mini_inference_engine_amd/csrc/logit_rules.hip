@@ -9,17 +9,25 @@
 // without z4 ever being in memory.
 //
 // A workgroup has a slice of one row's vocabulary.  It counts its slice's tokens in the LDS (one word a token: occurrences in the
-// output, and two bits for "in the text" and "has a bias"), by integer additions, whose order does not matter, then streams
-// the slice's logits past those words.  Every slice reads the row's whole text; it comes from the L2 for all slices but one.
+// output, and two bits for "in the text" and "has a bias"), by integer operations, whose order does not matter, then streams
+// the slice's logits, asked for before the text is read, past those words.  Every slice reads the row's whole text; it comes from the L2 for
+// all slices but one.  Biases are settled after that, the last of a token's entries first.
+//
+// What bounds it, of what a call cannot do without (MI355X): 256 rows of 128,256 with texts of 700 to 2,000 tokens chosen in 54 us, where
+// the 134 MB of logits take 26 at the rate of a large copy: reading alone, in this division, takes 34 with the join of the slices, texts 8, biases 6, masks 4,
+// noise on a quarter of the rows 5, and half of the waves' time is waiting for the four dependent loads that a workgroup begins with.
+// 192 rows with texts of 4,000 to 12,000 adjusted in 55 us, 40 for their 205 MB: reading every text 32 times is two fifths of the
+// instructions.  Tried and slower: slices of 8,192 on 512 threads (62 and 59 us); tokens with a word gathered in a list and taken by themselves (64
+// and 57); a bound on the noise by one logarithm before the exact two (63); text and list asked for before the words are cleared (62 and 79).
 #include "launch.hpp"
 #include "sampling.hpp"
 #pragma clang fp contract(off)      // the formulas' roundings, one by one
 
-// Two ways of dividing a row: slices of 4,096 tokens on workgroups of 256 threads, joined by a second launch, and the
-// whole row on a workgroup of 1,024 threads that goes through slices of 32,768.
+// Two ways of dividing a row: slices of 4,096 tokens on workgroups of 256 threads, and a row that is short in one slice on a workgroup
+// of 1,024 threads.
 constexpr int PART_THREADS = 256, ROW_THREADS = 1024;
-constexpr int ahead_of(int threads) { return threads == ROW_THREADS ? 8 : 4; }        // reads of four logits a thread and slice, all on their way at once
-constexpr int slice_of(int threads) { return threads * 4 * ahead_of(threads); }
+constexpr int AHEAD = 4;                               // reads of four logits a thread, all on their way at once
+constexpr int slice_of(int threads) { return threads * 4 * AHEAD; }
 // four numbers wherever they begin
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -63,14 +71,35 @@ __device__ __forceinline__ float apply_rules(float z, uint32_t w, const RowRules
   return z;
 }
 
-// Grid (workgroups a row, rows); a workgroup takes every gridDim.x-th slice.  CHOOSE: its best candidate to best_v, best_i [rows,
-// workgroups], or, of a row that has one workgroup, the token to ``chosen``; else the adjusted logits to ``out``.
+__device__ __forceinline__ unsigned long long pack_candidate(float v, int i) {
+  return ((unsigned long long)__float_as_uint(v) << 32) | (uint32_t)i;
+}
+
+// The token of the best of n candidates, for every lane of a wave.
+__device__ __forceinline__ int best_of_row(const unsigned long long* best, int n) {
+  float bv = -INFINITY;
+  int bi = 0x7FFFFFFF;
+  for (int i = threadIdx.x; i < n; i += 64) {
+    const unsigned long long c = __hip_atomic_load(&best[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sample_better(__uint_as_float((uint32_t)(c >> 32)), (int)(uint32_t)c, bv, bi);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float ov = __shfl_xor(bv, o, 64);
+    const int oi = __shfl_xor(bi, o, 64);
+    sample_better(ov, oi, bv, bi);
+  }
+  return bi == 0x7FFFFFFF ? 0 : bi;
+}
+
+// Grid (workgroups a row, rows); a workgroup takes every gridDim.x-th slice.  CHOOSE: its best candidate to best [rows, workgroups], or,
+// of a row that has one workgroup, the token to ``chosen``; else the adjusted logits to ``out``.  With ``arrived`` (a counter a
+// row, 0 before and after) the last workgroup of a row to arrive joins the row's candidates: one launch instead of two.
 template <bool CHOOSE, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == PART_THREADS ? (CHOOSE ? 8 : 5) : 4)
 rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float* out, long out_ld,
              const float* __restrict__ temperatures, const long long* __restrict__ seeds, const int* __restrict__ counters,
-             float* __restrict__ best_v, int* __restrict__ best_i, int* __restrict__ chosen) {
-  constexpr int AHEAD = ahead_of(THREADS);
+             unsigned long long* best, int* arrived, int* __restrict__ chosen) {
   extern __shared__ __align__(16) uint32_t words[];                   // [slice]
   __shared__ float wave_v[THREADS / 64];
   __shared__ int wave_i[THREADS / 64];
@@ -227,31 +256,35 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   }
   if ((tid & 63) == 0) { wave_v[tid >> 6] = bv; wave_i[tid >> 6] = bi; }
   __syncthreads();
+  if (tid >= 64) return;
+  int last = 0;
   if (tid == 0) {
     for (int i = 1; i < THREADS / 64; ++i) sample_better(wave_v[i], wave_i[i], bv, bi);
     if (gridDim.x == 1) {
       chosen[r] = bi == 0x7FFFFFFF ? 0 : bi;
     } else {
-      best_v[(size_t)r * gridDim.x + blockIdx.x] = bv;
-      best_i[(size_t)r * gridDim.x + blockIdx.x] = bi;
+      // Past the L2s, which workgroups on different dies do not share, by itself: a release of the whole L2 costs far more.
+      __hip_atomic_store(&best[(size_t)r * gridDim.x + blockIdx.x], pack_candidate(bv, bi), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (arrived) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // it is there before the row's counter says so
+        last = __hip_atomic_fetch_add(&arrived[r], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+      }
     }
+  }
+  if (!__shfl(last, 0, 64)) return;
+  asm volatile("" ::: "memory");
+  const int token = best_of_row(best + (size_t)r * gridDim.x, gridDim.x);
+  if (tid == 0) {
+    chosen[r] = token;
+    __hip_atomic_store(&arrived[r], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
 
 // The best of a row's slices, one wave a row.
 __global__ void __launch_bounds__(64)
-best_of_slices_kernel(const float* __restrict__ best_v, const int* __restrict__ best_i, int* __restrict__ chosen, int slices) {
-  const size_t r = blockIdx.x;
-  float bv = -INFINITY;
-  int bi = 0x7FFFFFFF;
-  for (int i = threadIdx.x; i < slices; i += 64) sample_better(best_v[r * slices + i], best_i[r * slices + i], bv, bi);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ov = __shfl_xor(bv, o, 64);
-    const int oi = __shfl_xor(bi, o, 64);
-    sample_better(ov, oi, bv, bi);
-  }
-  if (threadIdx.x == 0) chosen[r] = bi == 0x7FFFFFFF ? 0 : bi;
+best_of_slices_kernel(const unsigned long long* best, int* __restrict__ chosen, int slices) {
+  const int token = best_of_row(best + (size_t)blockIdx.x * slices, slices);
+  if (threadIdx.x == 0) chosen[blockIdx.x] = token;
 }
 
 // history[slot of the token's row, its position] = the token, of every token of a step.
@@ -270,11 +303,11 @@ record_tokens_kernel(int* __restrict__ history, long ld, int slots, int most, co
 
 MIE_EXPORT const char* logit_rules_last_error() { return g_mie_error; }
 
-// Workgroups a row: one where a single workgroup has the row in one slice and rows are few or short, since a second launch costs
-// more than it saves (choosing, us a call one after another, one workgroup a row / slices: 1 row of 5,000 15.0 / 19.2, 1 of 32,000
-// 15.2 / 19.3, 32 of 32,000 22.1 / 19.8, 7 of 50,261 29 / 19.5); else one for each slice.
+// Workgroups a row: one for rows of up to three slices, which one workgroup goes through in less time than several take to meet (choosing,
+// alone, one workgroup / slices: 1 to 256 rows of 5,000 12.9 to 15.1 us / 14.8 to 19.3, of 12,000 15.2 to 20.8 / 15.2 to 21.6, of 16,384 15.8 to
+// 24.1 / 14.7 to 22.4, of 32,000 19.8 to 36.4 / 14.2 to 29.6), else one for each slice.
 MIE_EXPORT int mie_rules_slices(int rows, int V) {
-  if (V <= slice_of(ROW_THREADS) / 2 || (V <= slice_of(ROW_THREADS) && rows <= 4)) return 1;
+  if (V <= 3 * slice_of(PART_THREADS)) return 1;
   return (V + slice_of(PART_THREADS) - 1) / slice_of(PART_THREADS);
 }
 
@@ -288,8 +321,8 @@ static int check_rules(const char* what, const Rules& r, int rows, int V, long l
 
 template <bool CHOOSE>
 static int launch_rules(const char* what, const float* logits, long ld, const Rules& rules, int rows, int V, float* out, long out_ld,
-                        const float* temperatures, const long long* seeds, const int* counters, float* best_v, int* best_i, int* chosen,
-                        hipStream_t stream) {
+                        const float* temperatures, const long long* seeds, const int* counters, unsigned long long* best, int* arrived,
+                        int* chosen, hipStream_t stream) {
   if (rows <= 0) return 0;
   if (check_rules(what, rules, rows, V, ld)) return -1;
   const int slices = mie_rules_slices(rows, V);
@@ -299,10 +332,10 @@ static int launch_rules(const char* what, const float* logits, long ld, const Ru
   auto* kernel = slices > 1 ? rules_kernel<CHOOSE, PART_THREADS> : rules_kernel<CHOOSE, ROW_THREADS>;
   if (lds > 65536 - 256 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, what)) return -1;
   hipLaunchKernelGGL(kernel, dim3(slices, rows), dim3(threads), lds, stream, logits, ld, rules, V, slice, out, out_ld, temperatures,
-                     seeds, counters, best_v, best_i, chosen);
+                     seeds, counters, best, arrived, chosen);
   MIE_CHECK_LAUNCH(what);
-  if (CHOOSE && slices > 1) {
-    hipLaunchKernelGGL(best_of_slices_kernel, dim3(rows), dim3(64), 0, stream, best_v, best_i, chosen, slices);
+  if (CHOOSE && slices > 1 && !arrived) {
+    hipLaunchKernelGGL(best_of_slices_kernel, dim3(rows), dim3(64), 0, stream, best, chosen, slices);
     MIE_CHECK_LAUNCH(what);
   }
   return 0;
@@ -321,10 +354,12 @@ MIE_EXPORT int mie_adjust_logits(const float* logits, long ld, RULE_ARGS, float*
   return launch_rules<false>("adjust_logits", logits, ld, RULES, rows, V, out, out_ld, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, stream);
 }
 
-// best_v, best_i: [rows, mie_rules_slices] (unused where that is one)
+// best: [rows, mie_rules_slices] and, unless null (a second launch then joins the slices), arrived: [rows], zero; both unused where there is one slice,
+// and nobody else's while the call runs.
 MIE_EXPORT int mie_choose_by_rules(const float* logits, long ld, RULE_ARGS, const float* temperatures, const long long* seeds,
-                                   const int* counters, float* best_v, int* best_i, int* chosen, int rows, int V, hipStream_t stream) {
-  return launch_rules<true>("sample", logits, ld, RULES, rows, V, nullptr, 0, temperatures, seeds, counters, best_v, best_i, chosen, stream);
+                                   const int* counters, unsigned long long* best, int* arrived, int* chosen, int rows, int V,
+                                   hipStream_t stream) {
+  return launch_rules<true>("sample", logits, ld, RULES, rows, V, nullptr, 0, temperatures, seeds, counters, best, arrived, chosen, stream);
 }
 
 MIE_EXPORT int mie_record_tokens(int* history, long ld, int slots, int most, const int* ids, const int* taken_from, const int* earlier,

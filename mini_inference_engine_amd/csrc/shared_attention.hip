@@ -702,7 +702,7 @@ MIE_EXPORT int mie_shared_attention(const void* q, long q_stride, const void* k_
                                     const int* items, int num_items, int column_tiles, const int* row_parts, int most_parts, int Hq, int Hkv,
                                     int page, float scale_log2, float sink_log2, const float* head_sinks, hipStream_t stream) {
   if (rows <= 0) return 0;
-  if (Hkv < 1 || Hq % Hkv || page < 16 || page % 16 || max_blocks < 1 || pages < 1)
+  if (Hkv < 1 || Hq < 1 || Hq % Hkv || page < 16 || page % 16 || page > 1 << 20 || max_blocks < 1 || pages < 1)
     MIE_FAIL("shared_prefix_attention: %d query heads, %d kv heads, pages of %d keys", Hq, Hkv, page);
   if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) MIE_FAIL("shared_prefix_attention: caches that do not begin on 16 bytes");
   if (!(scale_log2 > 0.f)) MIE_FAIL("shared_prefix_attention: the scale must be above 0");

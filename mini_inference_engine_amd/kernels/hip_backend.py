@@ -102,6 +102,7 @@ class HipBackend(KernelBackend):
         self._libs = {}
         self._units = None          # compute units
         self._shared_libs = {}      # of attention over shared keys, by head size
+        self._choice_spaces = {}    # workspaces of choosing under rules, by stream
         self._rule_slices = {}      # slices that choosing under rules cuts a row into, by rows and vocabulary
         self._zeros = None          # 256 zero bytes on the device, what masked loads of grouped products read
         self._lt_workspace = None   # device memory the library's product kernels may use
@@ -2124,14 +2125,28 @@ class HipBackend(KernelBackend):
             if len(self._rule_slices) >= 4096:
                 self._rule_slices.clear()
             self._rule_slices[(R, V)] = lib.mie_rules_slices(R, V)
-        slices, best = self._rule_slices[(R, V)], 0
-        if slices > 1:                  # every slice's best, value and token
-            workspace = torch.empty(2 * R * slices, dtype=torch.int32, device=logits.device)
-            best = workspace.data_ptr()
+        slices, best, arrived = self._rule_slices[(R, V)], 0, 0
+        if slices > 1:
+            if torch.cuda.is_current_stream_capturing():        # a graph may run beside anything: memory of its own, a launch more
+                workspace = torch.empty(R * slices, dtype=torch.int64, device=logits.device)
+                best = workspace.data_ptr()
+            else:
+                best, arrived = self._choice_workspace(R, slices)
         library.check(lib, lib.mie_choose_by_rules(
-            logits.data_ptr(), logits.stride(0) if R > 1 else V, *args, t, s, c, best,
-            best + 4 * R * slices, o, R, V, self._stream()))
+            logits.data_ptr(), logits.stride(0) if R > 1 else V, *args, t, s, c, best, arrived, o, R, V,
+            self._stream()))
         return out
+
+    def _choice_workspace(self, R, slices):
+        """Addresses of the candidates of a choice's slices and of the counters by which the last of them is known, of the current
+        stream's own: calls on one stream run one after another, and each leaves the counters at 0."""
+        stream = torch._C._cuda_getCurrentRawStream(self._device_index)
+        best, arrived = self._choice_spaces.get(stream, (None, None))
+        if best is None or best.numel() < R * slices or arrived.numel() < R:
+            best = torch.empty(max(R * slices, 8192), dtype=torch.int64, device=self.device)
+            arrived = torch.zeros(max(R, 256), dtype=torch.int32, device=self.device)
+            self._choice_spaces[stream] = best, arrived
+        return best.data_ptr(), arrived.data_ptr()
 
     def adjust_logits(self, logits, rules, out=None):
         R, V = self._check_logits("adjust_logits", logits)

@@ -323,3 +323,62 @@ def test_refused_results(ops):
     wide = torch.zeros((1, 64), device="cuda").expand(2, 64)          # rows on top of one another
     with pytest.raises((ValueError, RuntimeError), match="logits|leading"):
         ops.adjust_logits(wide, none, out=torch.zeros((2, 64), device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R, V", [(7, 50261), (300, 20001), (64, 128256)])
+def test_calls_one_after_another_and_on_two_streams(ops, R, V):
+    """The last workgroup of a row joins the row's slices, by counters that every call leaves as it found them: many calls, sizes that
+    change in between, two streams at once, against the choice from adjusted logits."""
+    rules = make(R, V, 50, 4, "cuda")
+    temps, seeds = torch.zeros(R, device="cuda"), torch.arange(R, device="cuda")
+    counters = torch.zeros(R, dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    inputs = [torch.randn((R, V), generator=g, device="cuda") for _ in range(4)]
+    wants = [ops.sample(ops.adjust_logits(x, rules), temps, seeds, counters) for x in inputs]
+    small = make(3, 33000, 5, 9, "cuda")
+    x_small = torch.randn((3, 33000), generator=g, device="cuda")
+    want_small = ops.sample(ops.adjust_logits(x_small, small), temps[:3], seeds[:3], counters[:3])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(60):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i % 4, ops.sample(inputs[i % 4], temps, seeds, counters, rules=rules)))
+            if i % 5 == 0:
+                got.append((-1, ops.sample(x_small, temps[:3], seeds[:3], counters[:3], rules=small)))
+    torch.cuda.synchronize()
+    for i, t in got:
+        assert torch.equal(t, want_small if i < 0 else wants[i])
+
+
+@pytest.mark.gpu
+def test_a_captured_choice_beside_calls(ops):
+    """Replays of two graphs on two streams beside calls on a third: each has memory of its own."""
+    R, V = 40, 40000
+    rules = make(R, V, 50, 4, "cuda")
+    temps, seeds = torch.zeros(R, device="cuda"), torch.arange(R, device="cuda")
+    counters = torch.zeros(R, dtype=torch.int32, device="cuda")
+    inputs = [torch.randn((R, V), generator=torch.Generator().manual_seed(i)).cuda() for i in range(3)]
+    wants = [ops.sample(ops.adjust_logits(x, rules), temps, seeds, counters) for x in inputs]
+    outs = [torch.zeros(R, dtype=torch.int32, device="cuda") for _ in range(2)]
+    graphs = []
+    for x, out in zip(inputs, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.sample(x, temps, seeds, counters, out=out, rules=rules)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            here = [ops.sample(inputs[2], temps, seeds, counters, rules=rules) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], wants[0]) and torch.equal(outs[1], wants[1]) and all(torch.equal(h, wants[2]) for h in here)
