@@ -13,6 +13,8 @@ import torch
 TILE = 64               # columns that a workgroup's four waves take with one tile of 16 each
 BLOCK_KEYS = 32
 LEAST_KEYS = 64         # of a cut: an item's start and its partial result cost about as much
+LEAST_WIDE_KEYS = 192   # the same of items of more than 64 columns in bfloat16, whose partial results are the larger (32 rows behind 2,000
+                        # keys: cuts of 64 keys 22 us, of 128 18.7, of 192 17.1, of 256 18.8)
 
 
 class SharedPrefixPlan:
@@ -68,7 +70,8 @@ class SharedPrefixPlan:
         parts = np.zeros(self.num_rows, dtype=np.int64)
         items, several = [], []
         for (row, columns, begin, end), t, c in zip(work, tiles, cost):
-            pieces = 1 if whole and share is None else -(-(end - begin) // max(LEAST_KEYS, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
+            least = LEAST_WIDE_KEYS if c == wider[1] and not float32 else LEAST_KEYS
+            pieces = 1 if whole and share is None else -(-(end - begin) // max(least, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
             size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
             rows = columns // G
             at = begin
