@@ -5,13 +5,24 @@
 // each part, parts join by their log-sum-exps m + log2 l.  A plan made on the host (kernels/shared_prefix.py) cuts a step into
 // items: columns x keys of one kv head.  A column is one query head of one row; the columns of an item over shared keys are the
 // group's query heads of up to 64 CT / G rows (G query heads a kv head), those of an item over a row's own keys are its G query heads.
-// One workgroup an item and kv head: its four waves bring the keys and values of 32 keys after 32 into the LDS by loads that write the
-// LDS directly, NST - 1 blocks ahead, and each wave takes 16 CT of the columns through all of them:
-//   S^T[key, column]  = K[key, d] . Q^T[d, column]        A = 16 keys, B = 16 columns (16x16x32 bfloat16, 16x16x4 float32)
+// One workgroup of four waves an item and kv head.  With v_mfma_f32_16x16x32_bf16 (float32: 16x16x4)
+//   S^T[key, column]  = K[key, d] . Q^T[d, column]        A = 16 keys, B = 16 columns
 //   O^T[dim, column] += V^T[dim, key] . P^T[key, column]
 // The scores come out with lane % 16 = column and 4 consecutive rows a lane group.  In bfloat16 the 32 keys are dealt to the two score
 // tiles' rows so that lane group g ends up with keys 8 g .. 8 g + 7, which is what the second product takes of both operands; in float32 every
-// one of the second product's steps of 4 keys takes one number of each lane group.  Probabilities never leave registers.
+// one of the second product's steps of 4 keys takes one number of each lane group.  Probabilities never leave registers; they are rounded to
+// bfloat16 for the second product as the operand of its kind, their sum is of what they were before.
+//
+// Keys and values come into the LDS by loads that write it directly, and the waves share the work out in one of two ways:
+//   more than 16 columns: all waves bring in a stage (64 keys, 32 where a key has more than 256 bytes), each takes 16 CT of the columns through it
+//   up to 16 columns: each wave brings in and takes every fourth 32 keys, and the waves join in the LDS at the end; with the first way one
+//   wave would compute and three wait (a row's 1,024 keys of 128 numbers 19.5 us, 12.8 this way, of 4,096 63.7 and 40.9).
+//
+// What bounds it (MI355X).  256 rows of 32 / 8 heads of 128 behind 8,192 shared keys with 1 to 1,024 of their own, 125 us: the 537 MB of own keys
+// alone take 89 (6.0 TB/s, more than a large copy), the 34 GFLOP over shared keys alone 67, most of it hidden neither by the other nor by two waves a
+// SIMD: vector instructions 30 % of the time, scalar ones 25, matrix instructions 21, the rest waiting in a chain of LDS reads, products and
+// softmax (a stage of 64 keys 1.3 us by itself).  8 rows behind 30,000 keys 32.5 us for 134 MB (4.1 TB/s).  32 rows behind 2,000 keys 20 us, 4 of them
+// the join: a workgroup's first loads, last stores and one stage take 7 us.
 #include "attention_bf16_common.hpp"
 #include "launch.hpp"
 #include <type_traits>
@@ -38,7 +49,7 @@ struct SharedItem {
   int col0;           // first of them that the item takes
   int key_begin, key_end;
   int part;           // which of its rows' partial results
-  int unused0, unused1;
+  int unused[2];
 };
 
 template <typename T, int CT>
@@ -69,9 +80,6 @@ struct Layout {
   static __device__ __forceinline__ int key_turn(int r) { return (ES == 2 ? (r & 3) | ((r >> 3 & 1) << 2) : r & 7) & TURN; }
   static __device__ __forceinline__ int value_turn(int d) { return ES == 2 ? d >> 2 & 1 : d >> 1 & 3; }
 };
-
-__device__ __forceinline__ float load_one(const float* p) { return *p; }
-__device__ __forceinline__ bf16 load_one(const bf16* p) { return *p; }
 
 template <typename T, int CT>
 __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 2 && D <= 128 ? 2 : 1)
@@ -261,7 +269,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
         } else {
           T e[16 / sizeof(T)];
 #pragma unroll
-          for (int j = 0; j < (int)(16 / sizeof(T)); ++j) e[j] = load_one(qp + d0 + j);
+          for (int j = 0; j < (int)(16 / sizeof(T)); ++j) e[j] = qp[d0 + j];
           __builtin_memcpy(&qf[ct][s].q, e, 16);
         }
       }

@@ -100,12 +100,13 @@ class SharedPrefixPlan:
     def _worth_it(self, G: int, units: int, float32: bool) -> bool:
         """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup a kv head, with no partial
         results and no second launch: as long as that takes no longer than the second launch costs.  Measured, us a call one after another,
-        whole / shared (4 heads of 64 and 8 of 128, 4 to 64 rows): 500 keys 11.8 / 16.5, 1,000 keys 11.7 / 16.5 and 11.7 to 16.8 / 16.4 to 19.1;
-        256 rows of 500 keys of 8 heads of 128 58 / 35; float32 500 keys 13 / 16.5 and 21 to 41 / 16.5 to 34, 200 keys 11.6 / 16.5 and 12 to 24 / 16.5
-        to 28."""
+        whole / shared.  4 kv heads of 64: 4 to 64 rows of 500 keys 11.6 / 16.1, of 1,000 11.7 / 16.1, 256 rows (two rounds of workgroups) of 500
+        17.5 / 23.4, of 1,000 21.6 / 25.9.  8 of 128: 4 to 64 rows of 500 keys 11.6 / 16.0, of 1,000 11.7 to 15.9 / 16.2 to 17.8, 256 rows of 200 28.8 /
+        36.3, of 500 39.4 / 38.6.  float32, 4 of 64: 200 keys 11.5 / 16.1, 500 keys 13.0 / 16.2, 1,000 keys 18.8 / 16.1; 8 of 128: 200 keys 12.0 to
+        23.7 / 15.9 to 28.3, 500 keys 21.3 to 41.0 / 15.8 to 32.1."""
         D, rounds = self.head_dim, -(-self.num_rows * self.num_kv_heads // (2 * units))
         if G > 16 or D % 32 or D * (4 if float32 else 2) > 512:
-            most = 128                              # one wave computes: see csrc/shared_attention.hip
+            most = 128                              # one wave of four computes: see csrc/shared_attention.hip
         else:
-            most = min(512, 32768 // D) if float32 else min(1024, 131072 // D)
+            most = min(512, 32768 // D) if float32 else min(1536, 131072 // D)
         return self.max_context * rounds > most
