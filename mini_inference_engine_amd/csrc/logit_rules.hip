@@ -23,10 +23,11 @@
 #include "sampling.hpp"
 #pragma clang fp contract(off)      // the formulas' roundings, one by one
 
-// Two ways of dividing a row: slices of 4,096 tokens on workgroups of 256 threads, and a row that is short in one slice on a workgroup
-// of 1,024 threads.
+// Two ways of dividing a row: slices of up to 4,096 tokens on workgroups of 256 threads, and a row that is short in one slice on a
+// workgroup of 1,024 threads.
 constexpr int PART_THREADS = 256, ROW_THREADS = 1024;
 constexpr int AHEAD = 4;                               // reads of four logits a thread, all on their way at once
+constexpr int ARRIVED = 32;                            // numbers from one row's counter to the next: a cache line each, so that rows do not wait for one another
 constexpr int slice_of(int threads) { return threads * 4 * AHEAD; }
 // four numbers wherever they begin
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -267,7 +268,7 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
       __hip_atomic_store(&best[(size_t)r * gridDim.x + blockIdx.x], pack_candidate(bv, bi), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       if (arrived) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // it is there before the row's counter says so
-        last = __hip_atomic_fetch_add(&arrived[r], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+        last = __hip_atomic_fetch_add(&arrived[(size_t)r * ARRIVED], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
       }
     }
   }
@@ -276,7 +277,7 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   const int token = best_of_row(best + (size_t)r * gridDim.x, gridDim.x);
   if (tid == 0) {
     chosen[r] = token;
-    __hip_atomic_store(&arrived[r], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&arrived[(size_t)r * ARRIVED], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
 
@@ -303,12 +304,21 @@ record_tokens_kernel(int* __restrict__ history, long ld, int slots, int most, co
 
 MIE_EXPORT const char* logit_rules_last_error() { return g_mie_error; }
 
-// Workgroups a row: one for rows of up to three slices, which one workgroup goes through in less time than several take to meet (choosing,
-// alone, one workgroup / slices: 1 to 256 rows of 5,000 12.9 to 15.1 us / 14.8 to 19.3, of 12,000 15.2 to 20.8 / 15.2 to 21.6, of 16,384 15.8 to
-// 24.1 / 14.7 to 22.4, of 32,000 19.8 to 36.4 / 14.2 to 29.6), else one for each slice.
+// Tokens a workgroup takes.  The whole of a short row, which one workgroup goes through in less time than several take to meet (choosing, alone, 1 to
+// 256 rows of 5,000: one workgroup 12.9 to 15.1 us, two slices 14.8 to 19.3).  Else slices, shorter ones as long as they are few: choosing from 1 row
+// of 32,000 18.1 us with slices of 4,096, 13.8 of 1,024, 32 rows 16.7 and 13.7, 64 rows 19.0 and (2,048) 16.6; four a compute unit are
+// enough, at eight every text is read too often (32 rows of 128,256 20.5 us, 23.8).
+static int slice_for(int rows, int V) {
+  if (V <= 2 * slice_of(PART_THREADS)) return (V + 3) & ~3;
+  int slice = slice_of(PART_THREADS);
+  while (slice > PART_THREADS * 4 && (long)rows * ((V + slice - 1) / slice) < 4L * mie_compute_units()) slice /= 2;
+  return slice;
+}
+
+// Workgroups a row.
 MIE_EXPORT int mie_rules_slices(int rows, int V) {
-  if (V <= 3 * slice_of(PART_THREADS)) return 1;
-  return (V + slice_of(PART_THREADS) - 1) / slice_of(PART_THREADS);
+  const int slice = slice_for(rows, V);
+  return (V + slice - 1) / slice;
 }
 
 static int check_rules(const char* what, const Rules& r, int rows, int V, long ld) {
@@ -325,9 +335,8 @@ static int launch_rules(const char* what, const float* logits, long ld, const Ru
                         int* chosen, hipStream_t stream) {
   if (rows <= 0) return 0;
   if (check_rules(what, rules, rows, V, ld)) return -1;
-  const int slices = mie_rules_slices(rows, V);
+  const int slice = slice_for(rows, V), slices = (V + slice - 1) / slice;
   const int threads = slices > 1 ? PART_THREADS : ROW_THREADS;
-  const int slice = V < slice_of(threads) ? (V + 3) & ~3 : slice_of(threads);
   const int lds = slice * 4;
   auto* kernel = slices > 1 ? rules_kernel<CHOOSE, PART_THREADS> : rules_kernel<CHOOSE, ROW_THREADS>;
   if (lds > 65536 - 256 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, what)) return -1;
@@ -354,7 +363,7 @@ MIE_EXPORT int mie_adjust_logits(const float* logits, long ld, RULE_ARGS, float*
   return launch_rules<false>("adjust_logits", logits, ld, RULES, rows, V, out, out_ld, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, stream);
 }
 
-// best: [rows, mie_rules_slices] and, unless null (a second launch then joins the slices), arrived: [rows], zero; both unused where there is one slice,
+// best: [rows, mie_rules_slices] and, unless null (a second launch then joins the slices), arrived: [32 rows], zero; both unused where there is one slice,
 // and nobody else's while the call runs.
 MIE_EXPORT int mie_choose_by_rules(const float* logits, long ld, RULE_ARGS, const float* temperatures, const long long* seeds,
                                    const int* counters, unsigned long long* best, int* arrived, int* chosen, int rows, int V,

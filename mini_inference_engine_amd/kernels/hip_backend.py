@@ -2142,9 +2142,9 @@ class HipBackend(KernelBackend):
         stream's own: calls on one stream run one after another, and each leaves the counters at 0."""
         stream = torch._C._cuda_getCurrentRawStream(self._device_index)
         best, arrived = self._choice_spaces.get(stream, (None, None))
-        if best is None or best.numel() < R * slices or arrived.numel() < R:
+        if best is None or best.numel() < R * slices or arrived.numel() < 32 * R:
             best = torch.empty(max(R * slices, 8192), dtype=torch.int64, device=self.device)
-            arrived = torch.zeros(max(R, 256), dtype=torch.int32, device=self.device)
+            arrived = torch.zeros(32 * max(R, 256), dtype=torch.int32, device=self.device)
             self._choice_spaces[stream] = best, arrived
         return best.data_ptr(), arrived.data_ptr()
 

@@ -84,7 +84,7 @@ def ops():
 
 
 SIZES = [(1, 1, 1), (1, 5, 3), (3, 31, 40), (2, 1023, 17), (5, 1024, 300), (4, 1025, 1), (2, 4099, 2000), (7, 50261, 700), (1, 128256, 5000),
-         (130, 33000, 100), (300, 20001, 257)]
+         (130, 33000, 100), (300, 20001, 257), (9, 8192, 50), (9, 8193, 50), (3, 12289, 4000)]
 
 
 @pytest.mark.gpu
