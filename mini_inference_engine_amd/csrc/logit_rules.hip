@@ -21,6 +21,7 @@
 // and 57); a bound on the noise by one logarithm before the exact two (63); text and list asked for before the words are cleared (62 and 79).
 #include "launch.hpp"
 #include "sampling.hpp"
+#include <type_traits>
 #pragma clang fp contract(off)      // the formulas' roundings, one by one
 
 // Two ways of dividing a row: slices of up to 4,096 tokens on workgroups of 256 threads, and a row that is short in one slice on a
@@ -106,45 +107,31 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   __shared__ int wave_i[THREADS / 64];
   const int r = blockIdx.y, tid = threadIdx.x;
 
-  RowRules row{1.f, 0.f, 0.f};
-  int length = 0, prompt = 0;
-  const int* text = nullptr;
-  if (rules.history) {
-    row.repetition = rules.repetition[r];
-    row.presence = rules.presence[r];
-    row.frequency = rules.frequency[r];
-    const int s = rules.slot[r];
-    if ((row.repetition != 1.f || row.presence != 0.f || row.frequency != 0.f) && s >= 0 && s < rules.slots) {
-      text = rules.history + (size_t)s * rules.history_ld;
-      length = clamp_int(rules.length[r], 0, rules.most);
-      prompt = clamp_int(rules.prompt[r], 0, length);
-    }
-  }
-  int listed = 0;
-  const int* list = nullptr;
-  const float* list_values = nullptr;
-  if (rules.bias_starts) {
-    const int a = clamp_int(rules.bias_starts[r], 0, rules.biases), b = clamp_int(rules.bias_starts[r + 1], a, rules.biases);
-    listed = b - a;
-    list = rules.bias_tokens + a;
-    list_values = rules.bias_values + a;
-  }
-  const uint32_t* mask = nullptr;
-  if (rules.masks) {
-    const int m = rules.mask_row[r];
-    if (m >= 0 && m < rules.num_masks) mask = rules.masks + (size_t)m * rules.mask_ld;
-  }
-  bool noisy = false;
-  float inv_t = 1.f;
+  // Everything a row says of itself is asked for at once, from the logits where a rule is absent (what is read there is not used): one wait
+  // and not one behind each test.
+  auto of_row = [&](const auto* p, int i) {
+    using N = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
+    return *(p ? p + i : reinterpret_cast<const N*>(logits));
+  };
+  RowRules row{of_row(rules.repetition, r), of_row(rules.presence, r), of_row(rules.frequency, r)};
+  const int in_slot = of_row(rules.slot, r), in_length = of_row(rules.length, r), in_prompt = of_row(rules.prompt, r);
+  const int bias_a = of_row(rules.bias_starts, r), bias_b = of_row(rules.bias_starts, r + 1), in_mask = of_row(rules.mask_row, r);
+  float temperature = 0.f;
   uint32_t key = 0;
   if (CHOOSE) {
-    const float t = temperatures[r];
-    noisy = t > 0.f;
-    if (noisy) {
-      inv_t = 1.0f / t;
-      key = sample_key((unsigned long long)seeds[r], counters[r]);
-    }
+    temperature = temperatures[r];
+    key = sample_key((unsigned long long)seeds[r], counters[r]);
   }
+  const bool penalised = rules.history && (row.repetition != 1.f || row.presence != 0.f || row.frequency != 0.f) && in_slot >= 0 && in_slot < rules.slots;
+  const int* text = penalised ? rules.history + (size_t)in_slot * rules.history_ld : nullptr;
+  const int length = penalised ? clamp_int(in_length, 0, rules.most) : 0, prompt = clamp_int(in_prompt, 0, length);
+  const int first_bias = rules.bias_starts ? clamp_int(bias_a, 0, rules.biases) : 0;
+  const int listed = rules.bias_starts ? clamp_int(bias_b, first_bias, rules.biases) - first_bias : 0;
+  const int* list = rules.bias_tokens + first_bias;
+  const float* list_values = rules.bias_values + first_bias;
+  const uint32_t* mask = rules.masks && in_mask >= 0 && in_mask < rules.num_masks ? rules.masks + (size_t)in_mask * rules.mask_ld : nullptr;
+  const bool noisy = CHOOSE && temperature > 0.f;
+  const float inv_t = noisy ? 1.0f / temperature : 1.f;
   float bv = -INFINITY;
   int bi = 0x7FFFFFFF;
   const bool counted = length > 0 || listed > 0;                      // (the same in the whole workgroup)
