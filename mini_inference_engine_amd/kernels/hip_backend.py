@@ -2025,11 +2025,14 @@ class HipBackend(KernelBackend):
             parts = torch.empty(plan.num_parts * Hq * (D + 1), dtype=torch.float32, device=qkv.device)
             at = parts.data_ptr()
         items, row_parts = plan.addresses
+        stream = self._stream()
+        if (stream.value or 0) != plan.stream:
+            plan.used_on(stream.value or 0)
         library.check(lib, lib.mie_shared_attention(
             qkv.data_ptr(), qkv.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _code(qkv.dtype), at,
             at + 4 * plan.num_parts * Hq * D, bt.data_ptr(), bt.shape[1], k_cache.shape[0], step.positions.data_ptr(), T,
             items, plan.num_items, plan.column_tiles, row_parts, plan.most_parts, Hq, Hkv, page,
-            scale * self.LOG2_E, sink_log2, head_sinks, self._stream()))
+            scale * self.LOG2_E, sink_log2, head_sinks, stream))
         return out
 
     LOG2_E = 1.4426950408889634

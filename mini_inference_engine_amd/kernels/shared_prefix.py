@@ -20,8 +20,8 @@ LEAST_WIDE_KEYS = 192   # the same of items of more than 64 columns in bfloat16,
 class SharedPrefixPlan:
     """Who shares what in a step of single-token rows.  ``groups``: (rows, keys) of every run of rows, in order; ``contexts``: the
     most keys each row has while the plan is used (its position + 1, or more: a plan holds for as many steps as its rows and
-    shared keys stay and their contexts suffice).  Made once a step, or once for many, and used by every layer of it; on another
-    stream than the one it was made on only once that has been waited for.  ``share``: whether shared keys are read once for all
+    shared keys stay and their contexts suffice; keys behind them are not seen).  Made once a step, or once for many, and used by every
+    layer of it, in captured graphs as well as long as it is kept, but not made while a stream records.  ``share``: whether shared keys are read once for all
     (True), by every row for itself (False), or what is faster (None)."""
 
     def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256,
@@ -92,10 +92,24 @@ class SharedPrefixPlan:
         self.join = self.most_parts != 1
         packed = np.concatenate([np.asarray(items, dtype=np.int32).reshape(-1), starts])
         data = torch.from_numpy(packed)
+        self.stream = self.ready = None             # where the plan was sent from, and the event behind its copy
         if torch.device(device).type == "cuda":
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("shared prefix: a plan is made before a capture, not in it (a replay would send its host memory again)")
+            stream = torch.cuda.current_stream(device)
             data = data.pin_memory().to(device, non_blocking=True)
+            self.stream, self.ready = stream.cuda_stream, torch.cuda.Event()
+            self.ready.record(stream)
+        self._data = data
         self.items, self.row_parts = data[:8 * len(items)], data[8 * len(items):]
         self.addresses = self.items.data_ptr(), self.row_parts.data_ptr()
+
+    def used_on(self, stream: int) -> None:
+        """The current stream, ``stream`` by handle, is about to read the plan: another than its own waits for it and keeps its memory."""
+        if stream != self.stream and self.ready is not None and not torch.cuda.is_current_stream_capturing():
+            here = torch.cuda.current_stream(self._data.device)
+            here.wait_event(self.ready)
+            self._data.record_stream(here)
 
     def _worth_it(self, G: int, units: int, float32: bool) -> bool:
         """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup a kv head, with no partial

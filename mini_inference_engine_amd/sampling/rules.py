@@ -53,6 +53,8 @@ class RuleInputs:
             pieces.append(np.asarray(numbers, dtype=dtype).view(np.int32))
 
         if any(p.has_penalties for p in params):
+            if history is None:
+                raise ValueError("penalties look at the requests' texts, which nobody keeps (ModelRunner.keep_token_history)")
             put("slots", [s.cache.state_slot for s in seqs])
             put("lengths", lengths)
             put("prompt_lengths", [s.prompt_len for s in seqs])

@@ -109,9 +109,10 @@ def test_adjusted_logits(ops, size):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("offset, stride", [(0, 1031), (1, 1032), (3, 1036), (4, 1036)])
-def test_adjusted_logits_of_rows_anywhere(ops, offset, stride):
-    R, V = 5, 1029
+@pytest.mark.parametrize("V", [1029, 20005])
+@pytest.mark.parametrize("offset, stride", [(0, 2), (1, 3), (3, 7), (4, 7)])
+def test_adjusted_logits_of_rows_anywhere(ops, V, offset, stride):
+    R, stride = 5, V + stride
     rules = make(R, V, 60, 9, "cuda")
     pool = torch.randn(R * stride + 8, generator=torch.Generator().manual_seed(2)).cuda()
     logits = pool[offset:offset + R * stride].view(R, stride)[:, :V]
@@ -119,6 +120,8 @@ def test_adjusted_logits_of_rows_anywhere(ops, offset, stride):
     out = out_pool[offset:offset + R * stride].view(R, stride)[:, :V]
     want, most = plain(logits, rules)
     check_adjusted(ops.adjust_logits(logits, rules, out=out), want, most)
+    temps, seeds, counters = torch.zeros(R, device="cuda"), torch.zeros(R, dtype=torch.int64, device="cuda"), torch.zeros(R, dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.sample(logits, temps, seeds, counters, rules=rules), ops.sample(out, temps, seeds, counters))
     mine = torch.zeros(R * stride + 8, dtype=torch.bool, device="cuda")
     mine[offset:offset + R * stride].view(R, stride)[:, :V] = True
     assert (out_pool[~mine] == 77.0).all()          # nothing beside the rows is written
@@ -320,6 +323,9 @@ def test_refused_results(ops):
     with pytest.raises(ValueError, match="logits"):
         ops.adjust_logits(logits.double(), none)
     assert ops.adjust_logits(logits[:0], none).shape == (0, 64)
+    nobody = torch.zeros(0, device="cuda")
+    for V in (64, 50000):
+        assert ops.sample(torch.zeros((0, V), device="cuda"), nobody, nobody.long(), nobody.to(torch.int32), rules=none).shape == (0,)
     wide = torch.zeros((1, 64), device="cuda").expand(2, 64)          # rows on top of one another
     with pytest.raises((ValueError, RuntimeError), match="logits|leading"):
         ops.adjust_logits(wide, none, out=torch.zeros((2, 64), device="cuda"))

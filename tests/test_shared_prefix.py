@@ -266,6 +266,59 @@ def test_in_a_graph_and_on_another_stream(ops):
 
 
 @pytest.mark.gpu
+def test_a_plan_on_other_streams_and_not_in_a_capture(ops):
+    """A plan made on one stream and used at once on another, thrown away while that still runs; none is made while a stream records."""
+    groups = [(12, 700), (4, 0)]
+    s = make(groups, [720 + i for i in range(12)] + [5, 90, 300, 719], 8, 2, 64, 16, BF16, poison=False)
+    step, group = step_of(s)
+    want = plain(s, 8, 2, 64, 0.125)
+    contexts = [p + 1 for p in s.positions.tolist()]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            plan = ops[BF16].plan_shared_prefix(groups, contexts, 8, 2, 64, share=True)
+        with torch.cuda.stream(streams[1 - i % 2]):
+            outs.append(ops[BF16].shared_prefix_attention(s.q, 8, 2, 64, s.k, s.v, group, step, 0.125, plan))
+        del plan
+    torch.cuda.synchronize()
+    for out in outs:
+        assert torch.equal(out, outs[0])
+    check(outs[0], *want, 64, BF16)
+    x = torch.zeros(8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="before a capture"):
+            ops[BF16].plan_shared_prefix(groups, contexts, 8, 2, 64, share=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 2, 48)])
+def test_table_entries_that_are_no_page(ops, heads, dtype):
+    """Beyond a row's own pages a block table may hold anything."""
+    groups = [(5, 96), (2, 0)]
+    s = make(groups, [96, 100, 130, 140, 97, 3, 40], *heads, 16, dtype)
+    s.tables = torch.cat([s.tables, torch.zeros((s.T, 9), dtype=torch.int32, device="cuda")], 1).contiguous()
+    for r, p in enumerate(s.positions.tolist()):
+        s.tables[r, p // 16 + 1:] = torch.tensor([-1, 2**31 - 1, -2**31, s.k.shape[0]], dtype=torch.int32).repeat(9)[:s.tables.shape[1] - p // 16 - 1].cuda()
+    run(ops, s, groups, *heads, dtype)
+    run(ops, s, groups, *heads, dtype, contexts=[200] * 7)
+
+
+@pytest.mark.gpu
+def test_a_step_of_no_rows(ops):
+    plan = ops[BF16].plan_shared_prefix([], [], 4, 2, 64)
+    assert (plan.num_items, plan.num_parts, plan.join) == (0, 0, False)
+    s = make([(1, 0)], [4], 4, 2, 64, 16, BF16)
+    step, group = step_of(s, most=0, num_rows=0, num_decode_rows=0, num_tokens=0, host={})
+    step.token_row, step.positions = step.token_row[:0], step.positions[:0]
+    assert ops[BF16].shared_prefix_attention(s.q[:0], 4, 2, 64, s.k, s.v, group, step, 0.1, plan).shape == (0, 256)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_pages_beyond_32_bits_of_offset(ops, dtype):
     Hq, Hkv, D, page = 4, 2, 128, 16
