@@ -557,7 +557,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[(wave * 16 + col) * (D + 1) + dt * 16 + 4 * kb + i] = O[0][dt][i] * f;
+        for (int i = 0; i < 4; ++i) s_o[(wave * 16 + col) * (D + 1) + dt * 16 + 4 * kb + i] = m[0] == -INFINITY ? 0.f : O[0][dt][i] * f;
       __syncthreads();
       for (int e = threadIdx.x; e < 16 * D; e += WAVES * 64) {
         const int hc = e / D, d = e - hc * D, c = col0 + hc;
@@ -595,6 +595,10 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     if (c >= columns) continue;
     const int r = first_row + c / G, head = kvh * G + c % G;
     const int slot = row_parts[r] + part;
+    if (sum == 0.f) {       // a column that sees nothing, beside others that may see a value which is no number: 0 times that is in its O
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) O[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     if (row_parts[r + 1] - row_parts[r] == 1) {             // nothing to join: the result itself
       const float sink = head_sinks ? head_sinks[head] * 1.4426950408889634f : sink_log2;
       const float total = sum + (sink == -INFINITY ? 0.f : m[ct] == -INFINITY ? 1.f : fast_exp2(sink - m[ct]));

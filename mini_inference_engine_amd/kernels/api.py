@@ -483,7 +483,8 @@ class KernelBackend:
     def shared_prefix_attention(self, qkv, num_q_heads, num_kv_heads, head_dim, k_cache, v_cache, group, step, scale, plan, sink=None):
         """``paged_attention`` (no window) of a step of single-token rows under ``plan``: the shared keys of a run are read through
         the block table of the run's first row and once for all its rows, the others through each row's own table.  A row at position p
-        sees keys 0 .. p; one at a position below 0 sees none and gives zeros.  ``scale`` > 0; ``sink`` as in ``paged_attention``.
+        sees keys 0 .. p; one at a position below 0 sees none and gives zeros; for one among its run's shared keys (it has fewer
+        than it was planned for) those keys' values must be finite numbers, also behind its own position.  ``scale`` > 0; ``sink`` as in ``paged_attention``.
         Returns [T, Hq * D] in act_dtype."""
         raise NotImplementedError
 

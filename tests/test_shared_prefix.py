@@ -184,6 +184,31 @@ def test_rows_that_see_nothing_give_zeros(ops, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads, n", [((8, 2, 64), 3), ((8, 2, 64), 24), ((16, 1, 48), 9), ((3, 3, 256), 5)])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+@pytest.mark.parametrize("keys", [32, 1024])
+def test_rows_that_see_nothing_beside_values_that_are_no_numbers(ops, keys, what, heads, n, dtype):
+    """What is among the shared values reaches the rows that see it and not the padding between them."""
+    Hq, Hkv, D = heads
+    groups, positions = [(n, keys)], [keys + 7 * i for i in range(n)]
+    s = make(groups, positions, *heads, 16, dtype)
+    none = [1, n - 1]
+    s.positions[none] = -1
+    s.v[s.tables[0, 1], 0, 3, 5] = what                    # key 21, dim 3 of kv head 0
+    step, group = step_of(s, most=max(positions) + 1)
+    for share in (True, False, None):
+        plan = ops[dtype].plan_shared_prefix(groups, [p + 1 for p in positions], *heads, share=share)
+        for sink in (None, 0.5):
+            got = ops[dtype].shared_prefix_attention(s.q, *heads, s.k, s.v, group, step, 0.1, plan, sink=sink).view(n, Hq, D).cpu()
+            assert (got[none] == 0).all()
+            got = got[[i for i in range(n) if i not in none]]
+            reached = torch.zeros_like(got, dtype=torch.bool)
+            reached[:, :Hq // Hkv, 3] = True
+            assert torch.equal(~torch.isfinite(got), reached)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_a_plan_serves_later_steps(ops, dtype):
     """Contexts planned ahead: the positions of the step decide what is seen."""
     groups = [(6, 90), (2, 0)]
