@@ -121,9 +121,9 @@ class LLMEngine:
         if params.seed is None:
             seq.seed = (self.cfg.seed << 32) ^ self._num_requests
         self._num_requests += 1
-        self.scheduler.add(seq)
         if params.has_penalties:
             self.runner.keep_token_history()
+        self.scheduler.add(seq)
         if params.allowed_tokens is not None:
             self._reading.add(seq)
         return seq

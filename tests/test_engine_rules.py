@@ -178,6 +178,39 @@ def test_where_nothing_is_allowed_the_request_ends(tiny_models):
         eng.generate(prompts_for(m, [6], seed=1), sp)
 
 
+def test_a_step_whose_rules_fail_can_be_taken_again(tiny_models):
+    """allowed_tokens that raises once, and once gives what is no token: the step is not taken, and the same one follows."""
+    m = tiny_models["A"]
+    want = run(m, "cpu", "float32", 1e-6, [dict(allowed_tokens=even_then_small), dict(repetition_penalty=1.4), dict()])[1]
+    calls = []
+
+    def sometimes(output):
+        calls.append(len(output))
+        if len(calls) == 3:
+            raise KeyError("not now")
+        return [10 ** 6] if len(calls) == 6 else even_then_small(output)
+
+    eng = engine(m, "cpu", "float32", num_blocks=40, max_num_seqs=6, max_num_batched_tokens=32)
+    seqs = [eng.add_request(p, SamplingParams(max_tokens=12, ignore_eos=True, **sp)) for p, sp in
+            zip(prompts_for(m, [5, 17, 33], seed=5), [dict(allowed_tokens=sometimes), dict(repetition_penalty=1.4), dict()])]
+    failed = []
+    while eng.has_work():
+        try:
+            eng.step()
+        except (KeyError, ValueError) as e:
+            failed.append(type(e))
+        eng.cache.check()
+    assert failed == [KeyError, ValueError] and len(calls) == 14
+    assert [s.output_ids for s in seqs] == want
+
+
+def test_a_refused_request_leaves_the_engine_as_it_was(tiny_models):
+    eng = engine(tiny_models["A"], "cpu", "float32", num_blocks=4, max_num_seqs=2, max_num_batched_tokens=32)
+    with pytest.raises(Exception, match="pages|blocks|tokens"):
+        eng.add_request([1] * 200, SamplingParams(max_tokens=300, repetition_penalty=1.5, allowed_tokens=even_then_small))
+    assert not eng.has_work() and not eng._reading
+
+
 def test_mask_words():
     w = mask_words([0, 31, 32, 99], 100)
     assert w.tolist() == [1 | -2**31, 1, 0, 8]
