@@ -16,7 +16,9 @@
 // Keys and values come into the LDS by loads that write it directly, and the waves share the work out in one of two ways:
 //   more than 16 columns: all waves bring in a stage (64 keys, 32 where a key has more than 256 bytes), each takes 16 CT of the columns through it
 //   up to 16 columns: each wave brings in and takes every fourth 32 keys, and the waves join in the LDS at the end; with the first way one
-//   wave would compute and three wait (a row's 1,024 keys of 128 numbers 19.5 us, 12.8 this way, of 4,096 63.7 and 40.9).
+//   wave would compute and three wait (a row's 1,024 keys of 128 numbers 19.5 us, 12.8 this way, of 4,096 63.7 and 40.9).  Of keys of more than 256
+//   bytes two waves take every second 32: their LDS then leaves room for a second workgroup (150 rows of 16 / 2 heads of 256 with up to 308 keys
+//   25.4 -> 16.7 us).  Where such items are many and short, each of these waves has one to itself, and nothing is joined in the LDS.
 //
 // What bounds it (MI355X).  256 rows of 32 / 8 heads of 128 behind 8,192 shared keys with 1 to 1,024 of their own, 125 us: the 537 MB of own keys
 // alone take 89 (6.0 TB/s, more than a large copy), the 34 GFLOP over shared keys alone 67, most of it hidden neither by the other nor by two waves a
@@ -28,8 +30,9 @@
 #include <type_traits>
 
 constexpr int WAVES = 4;
-// Tiles of 16 columns a wave: two, as far as their outputs have room in the registers.
-constexpr int mie_shared_most_tiles() { return D <= 128 ? 2 : 1; }
+// Tiles of 16 columns a wave: two in bfloat16, as far as their outputs have room in the registers.  (In float32 the matrix instructions bound what
+// many columns cost, and two workgroups on a compute unit do more than one of twice the columns.)
+constexpr int MOST_TILES = D <= 128 ? 2 : 1;
 
 // 16 bytes a lane from a lane's own address into the LDS at byte `at` + 16 lane (waits are the kernel's own)
 __device__ __forceinline__ void lane_load_to_lds(const char* from, uint32_t at) {
@@ -70,34 +73,38 @@ struct Layout {
   static constexpr int STAGE = H * 2 * TILE;
   static constexpr int STAGES = STAGE <= 8192 ? 6 : STAGE <= 16384 ? 4 : 2;
   // Items of up to 16 columns: each wave takes every fourth 32 keys, by itself, in slots of its own.
-  static constexpr bool APART = WHOLE && ROW <= 512;
+  static constexpr bool APART = WHOLE;
   static constexpr int SLOT = 2 * TILE;
-  static constexpr int SLOTS = STAGES * STAGE / (WAVES * SLOT) > 1 ? 2 : 1;
-  static constexpr int JOIN = WAVES * 16 * (D + 1) * 4;     // the waves' sums, where the slots were
-  static constexpr int LDS = !APART ? STAGES * STAGE : STAGES * STAGE > WAVES * SLOTS * SLOT ? (STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN)
-                                                                                             : (WAVES * SLOTS * SLOT > JOIN ? WAVES * SLOTS * SLOT : JOIN);
+  static constexpr int SHARERS = ROW <= 256 ? WAVES : 2;    // of the waves: two such workgroups have room on a compute unit
+  static constexpr int SLOTS = STAGES * STAGE / (SHARERS * SLOT) > 1 ? 2 : 1;
+  static constexpr int JOIN = SHARERS * 16 * (D + 1) * 4;     // the waves' sums, where the slots were
+  static constexpr int LDS = !APART ? STAGES * STAGE : STAGES * STAGE > SHARERS * SLOTS * SLOT ? (STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN)
+                                                                                             : (SHARERS * SLOTS * SLOT > JOIN ? SHARERS * SLOTS * SLOT : JOIN);
   // 16-byte places are turned by what tells the rows apart that are read at once, so that they lie in different banks
   static __device__ __forceinline__ int key_turn(int r) { return (ES == 2 ? (r & 3) | ((r >> 3 & 1) << 2) : r & 7) & TURN; }
   static __device__ __forceinline__ int value_turn(int d) { return ES == 2 ? d >> 2 & 1 : d >> 1 & 3; }
 };
 
 template <typename T, int CT>
-__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 2 && D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(WAVES * 64, D * sizeof(T) <= (CT == 1 ? 512 : 256) ? 2 : 1)
 shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
                         T* __restrict__ out, float* __restrict__ o_part, float* __restrict__ lse_part, const int* __restrict__ tables,
-                        int max_blocks, int pages, const int* __restrict__ positions, const SharedItem* __restrict__ items,
+                        int max_blocks, int pages, const int* __restrict__ positions, const SharedItem* __restrict__ items, int num_items, int whole_items,
                         const int* __restrict__ row_parts, int Hq, int Hkv, int page, float scale_log2, float sink_log2,
                         const float* __restrict__ head_sinks) {
   using L = Layout<T, CT>;
   constexpr bool HALF = sizeof(T) == 2;
   constexpr int QS = HALF ? KS : D / 16;                    // 16-byte pieces of a column's query that a lane holds
   extern __shared__ __align__(1024) char lds[];
-  const int item = blockIdx.x / Hkv, kvh = blockIdx.x - item * Hkv;
+  const int group = blockIdx.x / Hkv, kvh = blockIdx.x - group * Hkv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool solo = L::APART && group >= whole_items;       // every wave has an item of its own
+  const int item = solo ? whole_items + (group - whole_items) * L::SHARERS + wave : group;
+  if (item >= num_items || (solo && wave >= L::SHARERS)) return;
   const int first_row = items[item].first_row, columns = items[item].columns, col0 = items[item].col0;
   const int key_begin = items[item].key_begin, part = items[item].part;
   int key_end = items[item].key_end;
   const int G = Hq / Hkv;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kb = lane >> 4;
   // Keys that no other workgroup reads are loaded with the hint that nobody reads them again: they then push neither the shared keys nor
   // anything else out of the caches (256 rows behind 8,192 keys 177 -> 150 us, their own 1 to 1,024 keys alone 157 -> 97, 8 rows behind
@@ -108,7 +115,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     key_end = seen < key_end ? seen : key_end;
   }
 
-  const bool apart = L::APART && columns <= 16;             // the waves share out keys, not columns
+  const bool apart = L::APART && columns <= 16;             // the waves share out keys, or items, not columns
 
   // ---- the loads: unit u of 32 keys is 1 KB of their keys or values, a wave takes units wave, wave + 4, ..
   uint32_t rel[L::EACH];
@@ -138,7 +145,8 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
   const uint64_t page_bytes = (uint64_t)(uint32_t)Hkv * page * L::ROW;       // of keys; of values as well
   const char* const keys0 = reinterpret_cast<const char*>(k_cache) + (size_t)kvh * page * L::ROW;
   const char* const vals0 = reinterpret_cast<const char*>(v_cache) + (size_t)kvh * page * L::ROW;
-  const int stride = apart ? WAVES * BLOCK_KEYS : BLOCK_KEYS, blk1 = blk0 + (apart ? wave * BLOCK_KEYS : 0);
+  const bool deal = apart && !solo;
+  const int stride = deal ? L::SHARERS * BLOCK_KEYS : BLOCK_KEYS, blk1 = blk0 + (deal ? wave * BLOCK_KEYS : 0);
   const int more_pages = stride / page, more_off = stride % page;
   int index[2], off[2];
 #pragma unroll
@@ -215,7 +223,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
       for (int j = 0; j < KL; ++j) mie_load_to_lds_nt(v + (size_t)(j * dims) * page * L::ES, voff, to + L::TILE + t * half_bytes + j * 1024);
     }
   };
-  const int mine = apart ? (blocks - wave + WAVES - 1) / WAVES : 0;      // 32 keys each
+  const int mine = solo ? blocks : wave < L::SHARERS ? (blocks - wave + L::SHARERS - 1) / L::SHARERS : 0;      // of an item of up to 16 columns, 32 keys each
   Places next_own;
   if (apart) {
     if constexpr (L::APART) {
@@ -522,7 +530,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
     if (apart) {
       constexpr int VF = HALF ? DT : 2 * DT;
       for (int n = 0; n < mine; ++n) {
-        const int blk = blk1 + n * WAVES * BLOCK_KEYS;
+        const int blk = blk1 + n * stride;
         if (L::SLOTS == 2 && n + 1 < mine) MIE_VMCNT(L::UNITS);        // the wave's next 32 keys may still be on their way
         else MIE_VMCNT(0);
         asm volatile("" ::: "memory");
@@ -541,6 +549,8 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
         }
         attend_one(a, va, blk);
       }
+    }
+    if (deal) {
       // ---- the waves' columns are the same: join them in the LDS, once nobody reads or writes a slot
       __shared__ float s_m[WAVES][16], s_l[WAVES][16];
       float* s_o = reinterpret_cast<float*>(lds);
@@ -554,10 +564,11 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) M = fmaxf(M, s_m[w][col]);
       const float f = m[0] == -INFINITY ? 0.f : fast_exp2(m[0] - M);
+      if (wave < L::SHARERS)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[(wave * 16 + col) * (D + 1) + dt * 16 + 4 * kb + i] = m[0] == -INFINITY ? 0.f : O[0][dt][i] * f;
+          for (int i = 0; i < 4; ++i) s_o[(wave * 16 + col) * (D + 1) + dt * 16 + 4 * kb + i] = m[0] == -INFINITY ? 0.f : O[0][dt][i] * f;
       __syncthreads();
       for (int e = threadIdx.x; e < 16 * D; e += WAVES * 64) {
         const int hc = e / D, d = e - hc * D, c = col0 + hc;
@@ -566,7 +577,7 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) M1 = fmaxf(M1, s_m[w][hc]);
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
+        for (int w = 0; w < L::SHARERS; ++w) {
           total += s_m[w][hc] == -INFINITY ? 0.f : fast_exp2(s_m[w][hc] - M1) * s_l[w][hc];
           y += s_o[(w * 16 + hc) * (D + 1) + d];
         }
@@ -584,15 +595,17 @@ shared_attention_kernel(const T* __restrict__ q, long q_stride, int q_vec, const
       return;
     }
   }
-  if (CT == 2 && tiles == 2) walk(std::integral_constant<int, CT>());
-  else if (tiles > 0) walk(std::integral_constant<int, 1>());
-  else walk(std::integral_constant<int, 0>());
+  if (!solo) {
+    if (CT == 2 && tiles == 2) walk(std::integral_constant<int, CT>());
+    else if (tiles > 0) walk(std::integral_constant<int, 1>());
+    else walk(std::integral_constant<int, 0>());
+  }
 
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int c = col0 + (wave * CT + ct) * 16 + col;
+    const int c = col0 + ((solo ? 0 : wave * CT) + ct) * 16 + col;
     const float sum = quad_sum(l[ct]);
-    if (c >= columns) continue;
+    if (c >= columns || (solo && ct > 0)) continue;
     const int r = first_row + c / G, head = kvh * G + c % G;
     const int slot = row_parts[r] + part;
     if (sum == 0.f) {       // a column that sees nothing, beside others that may see a value which is no number: 0 times that is in its O
@@ -694,24 +707,26 @@ MIE_EXPORT int mie_shared_attention_head_dim() { return D; }
 
 template <typename T, int CT>
 static int launch_items(const void* q, long q_stride, const void* k_cache, const void* v_cache, void* out, float* o_part, float* lse_part,
-                        const int* tables, int max_blocks, int pages, const int* positions, const int* items, int num_items,
+                        const int* tables, int max_blocks, int pages, const int* positions, const int* items, int num_items, int whole_items,
                         const int* row_parts, int Hq, int Hkv, int page, float scale, float sink, const float* head_sinks, hipStream_t stream) {
   auto* kernel = shared_attention_kernel<T, CT>;
   constexpr int lds = Layout<T, CT>::LDS;
   if (lds > 65536 - 1024 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, "shared_prefix_attention")) return -1;
   const int q_vec = ((uintptr_t)q & 15) == 0 && (q_stride * (long)sizeof(T)) % 16 == 0;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)num_items * Hkv), dim3(WAVES * 64), lds, stream, (const T*)q, q_stride, q_vec,
+  constexpr int SOLO = Layout<T, CT>::SHARERS;
+  const unsigned groups = whole_items + (num_items - whole_items + SOLO - 1) / SOLO;
+  hipLaunchKernelGGL(kernel, dim3(groups * Hkv), dim3(WAVES * 64), lds, stream, (const T*)q, q_stride, q_vec,
                      (const T*)k_cache, (const T*)v_cache, (T*)out, o_part, lse_part, tables, max_blocks, pages, positions,
-                     (const SharedItem*)items, row_parts, Hq, Hkv, page, scale, sink, head_sinks);
+                     (const SharedItem*)items, num_items, whole_items, row_parts, Hq, Hkv, page, scale, sink, head_sinks);
   MIE_CHECK_LAUNCH("shared_prefix_attention");
   return 0;
 }
 
-// items [num_items, 8], row_parts [rows + 1]: the plan's; o_part [slots, Hq, D] and lse_part [slots, Hq] hold the partial results of rows
+// items [num_items, 8] (the first whole_items take a workgroup each, the others a wave each), row_parts [rows + 1]: the plan's; o_part [slots, Hq, D] and lse_part [slots, Hq] hold the partial results of rows
 // with several parts (slot row_parts[r] + part).  most_parts: the largest number of parts a row has, or 1 if every row has exactly one.  scale, sink: in units of log2 e.
 MIE_EXPORT int mie_shared_attention(const void* q, long q_stride, const void* k_cache, const void* v_cache, void* out, int dtype, float* o_part,
                                     float* lse_part, const int* tables, int max_blocks, int pages, const int* positions, int rows,
-                                    const int* items, int num_items, int column_tiles, const int* row_parts, int most_parts, int Hq, int Hkv,
+                                    const int* items, int num_items, int whole_items, int column_tiles, const int* row_parts, int most_parts, int Hq, int Hkv,
                                     int page, float scale_log2, float sink_log2, const float* head_sinks, hipStream_t stream) {
   if (rows <= 0) return 0;
   if (Hkv < 1 || Hq < 1 || Hq % Hkv || page < 16 || page % 16 || page > 1 << 20 || max_blocks < 1 || pages < 1)
@@ -722,11 +737,14 @@ MIE_EXPORT int mie_shared_attention(const void* q, long q_stride, const void* k_
   if (num_items > 0) {
     int rc;
 #define MIE_ITEMS(T, CT) launch_items<T, CT>(q, q_stride, k_cache, v_cache, out, o_part, lse_part, tables, max_blocks, pages, positions, items, \
-                                             num_items, row_parts, Hq, Hkv, page, scale_log2, sink_log2, head_sinks, stream)
-    constexpr int MOST = mie_shared_most_tiles();
-    if (column_tiles < 1 || column_tiles > MOST) MIE_FAIL("shared_prefix_attention: %d tiles of columns a wave, at most %d", column_tiles, MOST);
-    if (dtype == MIE_BF16) rc = column_tiles == MOST ? MIE_ITEMS(bf16, MOST) : MIE_ITEMS(bf16, 1);
-    else rc = column_tiles == MOST ? MIE_ITEMS(float, MOST) : MIE_ITEMS(float, 1);
+                                             num_items, whole_items, row_parts, Hq, Hkv, page, scale_log2, sink_log2, head_sinks, stream)
+    const int most = dtype == MIE_BF16 ? MOST_TILES : 1;
+    const int row_bytes = D * (dtype == MIE_BF16 ? 2 : 4);
+    if (whole_items < 0 || whole_items > num_items || (whole_items < num_items && row_bytes % 64))
+      MIE_FAIL("shared_prefix_attention: %d of %d items of a workgroup, heads of %d numbers", whole_items, num_items, D);
+    if (column_tiles < 1 || column_tiles > most) MIE_FAIL("shared_prefix_attention: %d tiles of columns a wave, at most %d", column_tiles, most);
+    if (dtype == MIE_BF16) rc = column_tiles == MOST_TILES ? MIE_ITEMS(bf16, MOST_TILES) : MIE_ITEMS(bf16, 1);
+    else rc = MIE_ITEMS(float, 1);
     if (rc) return rc;
   }
   if (most_parts != 1) {

@@ -2031,7 +2031,7 @@ class HipBackend(KernelBackend):
         library.check(lib, lib.mie_shared_attention(
             qkv.data_ptr(), qkv.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _code(qkv.dtype), at,
             at + 4 * plan.num_parts * Hq * D, bt.data_ptr(), bt.shape[1], k_cache.shape[0], step.positions.data_ptr(), T,
-            items, plan.num_items, plan.column_tiles, row_parts, plan.most_parts, Hq, Hkv, page,
+            items, plan.num_items, plan.whole_items, plan.column_tiles, row_parts, plan.most_parts, Hq, Hkv, page,
             scale * self.LOG2_E, sink_log2, head_sinks, stream))
         return out
 

@@ -173,7 +173,7 @@ register_kernel_module("prefill_attention_bf16", {
 }, variants=_head_variants, flags=["-mllvm", "-amdgpu-mfma-vgpr-form"])
 register_kernel_module("shared_attention", {
     "mie_shared_attention_head_dim": [],
-    "mie_shared_attention": [P, L, P, P, P, I, P, P, P, I, I, P, I, P, I, I, P, I, I, I, I, F, F, P, P],
+    "mie_shared_attention": [P, L, P, P, P, I, P, P, P, I, I, P, I, P, I, I, I, P, I, I, I, I, F, F, P, P],
 }, variants=_head_variants, flags=["-mllvm", "-amdgpu-mfma-vgpr-form"])
 # lt_gemm: host code only, the engine's own way into the library's matrix products (hipBLASLt) with the choice of
 # kernel per shape kept here.

@@ -2,7 +2,8 @@
 
 A step of single-token rows falls into runs of rows; the rows of a run share their first ``keys`` keys, read through the block
 table of the run's first row.  The plan cuts the step into items, each one workgroup a kv head (csrc/shared_attention.hip):
-columns (query heads of rows) x keys, so that all items take about the same time and there are as many as compute units.
+columns (query heads of rows) x keys, so that all items take about the same time and there are as many as compute units; the
+short items of single rows come last and get a wave each.
 An item leaves a partial result for each of its columns; a row's partial results are its items in order of keys.
 """
 from __future__ import annotations
@@ -13,8 +14,15 @@ import torch
 TILE = 64               # columns that a workgroup's four waves take with one tile of 16 each
 BLOCK_KEYS = 32
 LEAST_KEYS = 64         # of a cut: an item's start and its partial result cost about as much
+START = 500             # what a workgroup's start and end cost, in keys of an item of up to 16 columns
 LEAST_WIDE_KEYS = 192   # the same of items of more than 64 columns in bfloat16, whose partial results are the larger (32 rows behind 2,000
                         # keys: cuts of 64 keys 22 us, of 128 18.7, of 192 17.1, of 256 18.8)
+
+
+def _sharers(head_dim: int, float32: bool) -> int:
+    """How many of a workgroup's waves share the keys of an item of up to 16 columns, or have such items of their own; 0: one wave takes all its keys."""
+    row_bytes = head_dim * (4 if float32 else 2)
+    return 0 if row_bytes % 64 else 4 if row_bytes <= 256 else 2
 
 
 class SharedPrefixPlan:
@@ -55,26 +63,37 @@ class SharedPrefixPlan:
             work += [(r, G, k, contexts[r]) for r in range(first, first + n) if contexts[r] > k]
             first += n
         widest = max((w[1] for w in work), default=1)
-        self.column_tiles = 2 if widest > TILE and head_dim <= 128 else 1
+        self.column_tiles = 2 if widest > TILE and head_dim <= 128 and not float32 else 1
         wide = TILE * self.column_tiles
         tiles = [-(-w[1] // wide) for w in work]
         # What a key of an item costs, in keys of an item of up to 16 columns, whose waves share out the keys: measured, us for 64 keys in
-        # bfloat16 0.4, of up to 64 columns 0.9, of 128 columns 1.3 (head size 128); the 32-bit products of float32 weigh more.
-        wider = (4, 8) if float32 else (2, 3)
-        cost = [1 if w[1] <= 16 else wider[min(w[1], wide) > TILE] for w in work]
+        # bfloat16 0.4, of up to 64 columns 0.9, of 128 columns 1.3 (head size 128); the products of float32 weigh more.
+        wider = 4 if float32 else 2
+        cost = [1 if w[1] <= 16 else wider if min(w[1], wide) <= TILE else 3 for w in work]
         total = sum(t * c * (w[3] - w[2]) for w, t, c in zip(work, tiles, cost)) * num_kv_heads
         # One compute unit's share.  Items of half of it balance better and leave twice the partial results: over fifteen shapes in
         # geometric mean 35.3 us, 33.2 at two thirds, 31.9 at this, 33.9 at four thirds.
         most = -(-total // units)
 
         parts = np.zeros(self.num_rows, dtype=np.int64)
-        items, several = [], []
+        items, several, solo = [], [], []
+        # Rows whose own keys are few next to a compute unit's share get a wave each: fewer workgroups, and nothing to join among the waves.  (236
+        # rows of 48 / 6 heads of 64 behind 2,466 keys with 1 to 75 of their own 40.4 -> 37.8 us, 248 rows of 21 / 7 of 256 behind some 770 with
+        # 1 to 63 79 -> 53; eighty drawn shapes of heads up to 128 in geometric mean 8.76 -> 8.63, sixty of float32 or heads of 256 16.2 -> 14.6; the 256 rows below 131 -> 116.
+        # Twice as many keys in a wave are as good on the drawn shapes, half as many 1 % slower.)
+        sharers = _sharers(head_dim, float32) if G <= 16 else 0
+        share_with_starts = sum(t * (c * (w[3] - w[2]) + START) for w, t, c in zip(work, tiles, cost)) * num_kv_heads / units
+        few = (share_with_starts - START) / (2 * sharers) if sharers else 0
         for (row, columns, begin, end), t, c in zip(work, tiles, cost):
-            least = LEAST_WIDE_KEYS if c == wider[1] and not float32 else LEAST_KEYS
+            least = LEAST_WIDE_KEYS if c == 3 else LEAST_KEYS
             pieces = 1 if whole and share is None else -(-(end - begin) // max(least, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
             size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
             rows = columns // G
             at = begin
+            if rows == 1 and pieces == 1 and end - begin <= few:
+                solo.append((row, columns, 0, begin, end, int(parts[row]), 0, 0))
+                parts[row] += 1
+                continue
             while at < end:
                 # cuts lie on whole blocks of the cache, so that no block is read twice
                 to = end if end - at <= size else (at + size) // BLOCK_KEYS * BLOCK_KEYS
@@ -84,6 +103,8 @@ class SharedPrefixPlan:
         # the longest first: items of many columns take several times what those of one row do (256 rows behind 8,192 keys: the two kinds
         # spread among one another 256 us, these first 182)
         items = several + items
+        self.whole_items = len(items)               # of a workgroup each; those of a wave each come after them, waves of like length side by side
+        items += sorted(solo, key=lambda i: i[3] - i[4])
         self.num_items = len(items)
         starts = np.zeros(self.num_rows + 1, dtype=np.int32)
         np.cumsum(parts, out=starts[1:])
@@ -112,15 +133,23 @@ class SharedPrefixPlan:
             self._data.record_stream(here)
 
     def _worth_it(self, G: int, units: int, float32: bool) -> bool:
-        """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup a kv head, with no partial
-        results and no second launch: as long as that takes no longer than the second launch costs.  Measured, us a call one after another,
-        whole / shared.  4 kv heads of 64: 4 to 64 rows of 500 keys 11.6 / 16.1, of 1,000 11.7 / 16.1, 256 rows (two rounds of workgroups) of 500
-        17.5 / 23.4, of 1,000 21.6 / 25.9.  8 of 128: 4 to 64 rows of 500 keys 11.6 / 16.0, of 1,000 11.7 to 15.9 / 16.2 to 17.8, 256 rows of 200 28.8 /
-        36.3, of 500 39.4 / 38.6.  float32, 4 of 64: 200 keys 11.5 / 16.1, 500 keys 13.0 / 16.2, 1,000 keys 18.8 / 16.1; 8 of 128: 200 keys 12.0 to
-        23.7 / 15.9 to 28.3, 500 keys 21.3 to 41.0 / 15.8 to 32.1."""
-        D, rounds = self.head_dim, -(-self.num_rows * self.num_kv_heads // (2 * units))
-        if G > 16 or D % 32 or D * (4 if float32 else 2) > 512:
-            most = 128                              # one wave of four computes: see csrc/shared_attention.hip
+        """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup a kv head or one wave, with no
+        partial results and no second launch: as long as that takes no longer than the second launch costs.  Measured, us a call one after
+        another, whole / shared, rows from 4 to 64 and 256 of them.
+          4 kv heads of 64: 500 keys 12.7 / 17.3 and 14.3 / 18.0, 1,000 keys 12.5 / 17.3 and 21.9 / 20.6, 1,500 keys 12.6 / 17.3 and 30.8 / 23.2
+          8 of 128: 350 keys 12.6 / 17.3 and 22.0 / 25.2, 500 keys 12.6 / 17.5 and 24.2 / 26.4, 1,000 keys 12.6 to 16.2 / 17.6 and 42.3 / 26.8
+          4 of 256: 350 keys 13.7 / 17.5 and 25.7 / 29.7, 500 keys 16.6 / 17.5 and 30.9 / 28.7, 1,000 keys 24 / 18.5 and 53 / 29
+          float32, 4 of 64: 350 keys 12.6 / 17.5 and 22.6 / 23.4, 700 keys 14.8 / 17.7 and 38.4 / 30.9, 1,000 keys 17.9 / 17.4 and 51.5 / 35.6
+          8 of 128: 100 keys 12.6 to 16.1 / 17.4 and 47 / 39, 200 keys 17 to 24 / 17.6 and 74 / 42;  4 of 256: 100 keys 20 / 22 and 60 / 45
+          one wave takes all keys: 4 heads of 48: 350 keys 12.6 / 17.5 and 18.9 / 17.4, 700 keys 15.8 / 17.4 and 30.3 / 17.3;
+          2 heads of 128 with 20 query heads each: 500 keys 14.9 / 17.4 and 18.1 / 29.9, 700 keys 18.3 / 17.7 and 22.1 / 29.6,
+          float32 100 keys 15.2 / 17.2 and 22.8 / 32, 200 keys 22.6 / 17.6 and 34.9 / 37"""
+        D, load = self.head_dim, self.num_rows * self.num_kv_heads / units
+        sharers = _sharers(D, float32)
+        if G > 16 or not sharers:
+            most, load = 16384 // D if float32 else min(640, 81920 // D), load / 2
+        elif float32:
+            most, load = min(1536, 14400 * sharers // D), load * 2 / sharers
         else:
-            most = min(512, 32768 // D) if float32 else min(1536, 131072 // D)
-        return self.max_context * rounds > most
+            most, load = min(1536, 131072 // D), load / 3
+        return self.max_context * max(1, load) > most

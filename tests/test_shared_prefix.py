@@ -248,7 +248,7 @@ def test_long_prefix_many_rows(ops, dtype):
     groups = [(70, 5000), (1, 0), (33, 2049)]
     s = make(groups, rows_behind(groups, 400, 3), 8, 2, 128, 16, dtype, poison=False)
     out, plan = run(ops, s, groups, 8, 2, 128, dtype)
-    assert plan.column_tiles == 2 and plan.join
+    assert plan.column_tiles == (2 if dtype == BF16 else 1) and plan.join
 
 
 @pytest.mark.gpu
