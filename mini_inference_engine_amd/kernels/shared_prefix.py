@@ -72,18 +72,23 @@ class SharedPrefixPlan:
         cost = [1 if w[1] <= 16 else wider if min(w[1], wide) <= TILE else 3 for w in work]
         total = sum(t * c * (w[3] - w[2]) for w, t, c in zip(work, tiles, cost)) * num_kv_heads
         # One compute unit's share.  Items of half of it balance better and leave twice the partial results: over fifteen shapes in
-        # geometric mean 35.3 us, 33.2 at two thirds, 31.9 at this, 33.9 at four thirds.
+        # geometric mean 35.3 us, 33.2 at two thirds, 31.9 at this, 33.9 at four thirds.  But two workgroups on a unit do 1.35 times what one does, which
+        # long items are worth cutting for (two thirds: 256 rows behind 8,192 keys 118 -> 109 us, 77 of 56 / 7 heads of 32 behind 20,855 63 -> 53).
         most = -(-total // units)
+        if most > 3000:
+            most = -(-2 * most // 3)
 
         parts = np.zeros(self.num_rows, dtype=np.int64)
         items, several, solo = [], [], []
         # Rows whose own keys are few next to a compute unit's share get a wave each: fewer workgroups, and nothing to join among the waves.  (236
         # rows of 48 / 6 heads of 64 behind 2,466 keys with 1 to 75 of their own 40.4 -> 37.8 us, 248 rows of 21 / 7 of 256 behind some 770 with
-        # 1 to 63 79 -> 53; eighty drawn shapes of heads up to 128 in geometric mean 8.76 -> 8.63, sixty of float32 or heads of 256 16.2 -> 14.6; the 256 rows below 131 -> 116.
-        # Twice as many keys in a wave are as good on the drawn shapes, half as many 1 % slower.)
+        # 1 to 63 79 -> 53; the 256 rows below 131 -> 116; 220 rows of 15 / 5 of 128 with 200 to 220 keys, whole, 20 -> 15, with 800 39 -> 43.)  Of
+        # more workgroups than there is room for at once, the rows with up to 448 keys at any rate.
         sharers = _sharers(head_dim, float32) if G <= 16 else 0
         share_with_starts = sum(t * (c * (w[3] - w[2]) + START) for w, t, c in zip(work, tiles, cost)) * num_kv_heads / units
         few = (share_with_starts - START) / (2 * sharers) if sharers else 0
+        if sharers and sum(w[1] == G for w in work) * num_kv_heads > 2 * units:
+            few = max(few, 224 if float32 and sharers < 4 else 448)
         for (row, columns, begin, end), t, c in zip(work, tiles, cost):
             least = LEAST_WIDE_KEYS if c == 3 else LEAST_KEYS
             pieces = 1 if whole and share is None else -(-(end - begin) // max(least, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
@@ -133,23 +138,22 @@ class SharedPrefixPlan:
             self._data.record_stream(here)
 
     def _worth_it(self, G: int, units: int, float32: bool) -> bool:
-        """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup a kv head or one wave, with no
-        partial results and no second launch: as long as that takes no longer than the second launch costs.  Measured, us a call one after
-        another, whole / shared, rows from 4 to 64 and 256 of them.
-          4 kv heads of 64: 500 keys 12.7 / 17.3 and 14.3 / 18.0, 1,000 keys 12.5 / 17.3 and 21.9 / 20.6, 1,500 keys 12.6 / 17.3 and 30.8 / 23.2
-          8 of 128: 350 keys 12.6 / 17.3 and 22.0 / 25.2, 500 keys 12.6 / 17.5 and 24.2 / 26.4, 1,000 keys 12.6 to 16.2 / 17.6 and 42.3 / 26.8
-          4 of 256: 350 keys 13.7 / 17.5 and 25.7 / 29.7, 500 keys 16.6 / 17.5 and 30.9 / 28.7, 1,000 keys 24 / 18.5 and 53 / 29
-          float32, 4 of 64: 350 keys 12.6 / 17.5 and 22.6 / 23.4, 700 keys 14.8 / 17.7 and 38.4 / 30.9, 1,000 keys 17.9 / 17.4 and 51.5 / 35.6
-          8 of 128: 100 keys 12.6 to 16.1 / 17.4 and 47 / 39, 200 keys 17 to 24 / 17.6 and 74 / 42;  4 of 256: 100 keys 20 / 22 and 60 / 45
-          one wave takes all keys: 4 heads of 48: 350 keys 12.6 / 17.5 and 18.9 / 17.4, 700 keys 15.8 / 17.4 and 30.3 / 17.3;
-          2 heads of 128 with 20 query heads each: 500 keys 14.9 / 17.4 and 18.1 / 29.9, 700 keys 18.3 / 17.7 and 22.1 / 29.6,
-          float32 100 keys 15.2 / 17.2 and 22.8 / 32, 200 keys 22.6 / 17.6 and 34.9 / 37"""
+        """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup or wave a kv head, with no
+        partial results and no second launch: as long as that takes no longer.  Measured, us, whole / shared by (rows x kv heads) / 256; a
+        caller that launches one call after another adds to the second up to 17, which its two launches take from the host.
+          bfloat16, heads of 64:   1 to 2: 1,500 keys 10 to 14 / 14;   3: 800 keys 17 / 14;   4.3: 400 keys 16 / 15;   8: 400 keys 15 / 19, 800 25 / 21
+          of 128:    1 to 2: 800 keys 11 to 14 / 15 to 17;   3: 400 keys 15 / 17, 800 24 / 20;   4.3: 200 keys 15 / 18, 400 23 / 20;   8: 400 keys 21 / 27, 800 35 / 27
+          of 256:    1 to 2: 400 keys 15 to 20 / 15 to 22;   3: 200 keys 17 / 25, 400 24 / 26;   4.3: 100 keys 22 / 25, 200 32 / 27;   8: 200 keys 35 / 37
+          float32, of 64:   1: 800 keys 17 / 13;   2: 400 keys 16 / 13;   3: 200 keys 16 / 14;   4.3: 100 keys 16 / 14, 200 23 / 18;   8: 200 keys 24 / 27
+          of 128:    1: 200 keys 17 / 14;   2: 100 keys 16 / 16;   3: 30 keys 16 / 20, 100 25 / 18;   4.3: 30 keys 22 / 28;   8: 30 keys 31 / 40, 100 47 / 39
+          one wave takes all keys, 4 heads of 48: 0.1 to 1: 500 keys 12 / 7 to 11, 700 15 to 16 / 7 to 11;   4: 200 keys 14 / 15, 350 18 / 15
+          2 heads of 128 with 20 query heads each: 0.5: 500 keys 15 / 16;   2: 700 keys 22 / 29;   float32: 0.5: 100 keys 15 / 15, 200 23 / 18"""
         D, load = self.head_dim, self.num_rows * self.num_kv_heads / units
         sharers = _sharers(D, float32)
         if G > 16 or not sharers:
-            most, load = 16384 // D if float32 else min(640, 81920 // D), load / 2
+            most, rounds = 16384 // D if float32 else min(640, 81920 // D), load / 2
         elif float32:
-            most, load = min(1536, 14400 * sharers // D), load * 2 / sharers
+            most, rounds = 14400 * sharers // D, min(load, max(4, load / 2))
         else:
-            most, load = min(1536, 131072 // D), load / 3
-        return self.max_context * max(1, load) > most
+            most, rounds = min(1536, 131072 // D), -(-load // 2) if load <= 6 else 0.3 * load
+        return self.max_context * max(1, rounds) > most
