@@ -101,9 +101,10 @@ class HipBackend(KernelBackend):
             raise RuntimeError("no GPU visible to torch: the engine needs an MI355X (gfx950)")
         self._libs = {}
         self._units = None          # compute units
-        self._shared_libs = {}      # of attention over shared keys, by head size
+        self._direct = None         # the library of csrc/direct_calls.hip, and the entry points handed to it
+        self._choose_entries = self._adjust_entry = None
+        self._shared_libs = {}      # of attention over shared keys, by head size, with the entry point's address
         self._choice_spaces = {}    # workspaces of choosing under rules, by stream
-        self._rule_slices = {}      # slices that choosing under rules cuts a row into, by rows and vocabulary
         self._zeros = None          # 256 zero bytes on the device, what masked loads of grouped products read
         self._lt_workspace = None   # device memory the library's product kernels may use
         self._lt_rows = set()       # row counts whose library products get their kernel chosen by timing (prefer_rows)
@@ -124,6 +125,12 @@ class HipBackend(KernelBackend):
     def _stream(self) -> c_void_p:
         # the handle alone: building torch's Stream object costs several microseconds a launch
         return c_void_p(torch._C._cuda_getCurrentRawStream(self._device_index))
+
+    def _entry(self, lib, name: str):
+        """The address of an entry point that csrc/direct_calls.hip calls, and that library loaded."""
+        if self._direct is None:
+            self._direct = self.lib("direct_calls")
+        return ctypes.cast(getattr(lib, name), c_void_p).value
 
     def _on_device(self, *tensors) -> None:
         for t in tensors:
@@ -2006,6 +2013,18 @@ class HipBackend(KernelBackend):
         Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim
         if isinstance(qkv, ProjectionSums):
             qkv = qkv.finish()
+        stream = torch._C._cuda_getCurrentRawStream(self._device_index)
+        lib, entry = self._shared_libs.get(D, (None, None))
+        if (entry is not None and type(plan) is SharedPrefixPlan and (plan.num_q_heads, plan.num_kv_heads, plan.head_dim) == (Hq, Hkv, D)
+                and step.num_decode_rows == step.num_rows == plan.num_rows and step.max_context <= plan.max_context and not plan.exceeded_by(step)):
+            if stream != plan.stream:
+                plan.used_on(stream)
+            heads = isinstance(sink, torch.Tensor)
+            out = self._direct.mie_direct_shared(
+                entry, self._device_index, qkv, k_cache, v_cache, group.block_tables, step.positions, step.token_row, plan.numbers, scale,
+                float("-inf") if sink is None or heads else float(sink) * self.LOG2_E, sink if heads else None, stream)
+            if out is not None:
+                return out
         T, page, bt = self._check_shared(qkv, Hq, Hkv, D, k_cache, v_cache, group, step, scale, plan)
         dev = self._device_index
         for t in (qkv, k_cache, v_cache, bt, step.positions, plan.items):
@@ -2016,23 +2035,22 @@ class HipBackend(KernelBackend):
             head_sinks = _rules_vector("shared_prefix_attention", "sink", sink, torch.float32, Hq, dev)
         elif sink is not None:
             sink_log2 = float(sink) * self.LOG2_E
-        lib = self._shared_libs.get(D)
         if lib is None:
-            lib = self._shared_libs[D] = self.lib("shared_attention", (f"-DHEAD_DIM={D}",))
+            lib = self.lib("shared_attention", (f"-DHEAD_DIM={D}",))
+            self._shared_libs[D] = lib, self._entry(lib, "mie_shared_attention")
         out = torch.empty((T, Hq * D), dtype=qkv.dtype, device=qkv.device)
         at = 0
         if plan.join:               # partial outputs, then their log-sum-exps
             parts = torch.empty(plan.num_parts * Hq * (D + 1), dtype=torch.float32, device=qkv.device)
             at = parts.data_ptr()
         items, row_parts = plan.addresses
-        stream = self._stream()
-        if (stream.value or 0) != plan.stream:
-            plan.used_on(stream.value or 0)
+        if stream != plan.stream:
+            plan.used_on(stream)
         library.check(lib, lib.mie_shared_attention(
             qkv.data_ptr(), qkv.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _code(qkv.dtype), at,
             at + 4 * plan.num_parts * Hq * D, bt.data_ptr(), bt.shape[1], k_cache.shape[0], step.positions.data_ptr(), T,
             items, plan.num_items, plan.whole_items, plan.column_tiles, row_parts, plan.most_parts, Hq, Hkv, page,
-            scale * self.LOG2_E, sink_log2, head_sinks, stream))
+            scale * self.LOG2_E, sink_log2, head_sinks, c_void_p(stream)))
         return out
 
     LOG2_E = 1.4426950408889634
@@ -2050,8 +2068,7 @@ class HipBackend(KernelBackend):
         if plan.max_context > bt.shape[1] * page or step.max_context > plan.max_context:
             raise ValueError(f"shared_prefix_attention: a plan for contexts up to {plan.max_context}; the step's reach {step.max_context}, "
                              f"its block tables {bt.shape[1]} pages of {page}")
-        ends = step.host.get("row_context") if step.host else None
-        if ends is not None and (ends > plan.contexts).any():
+        if plan.exceeded_by(step):
             raise ValueError("shared_prefix_attention: a row's context is beyond the one it was planned for")
         if not 0 < scale < float("inf"):
             raise ValueError(f"shared_prefix_attention: scale {scale}")
@@ -2112,6 +2129,12 @@ class HipBackend(KernelBackend):
         return out
 
     def _choose_by_rules(self, logits, temperatures, seeds, counters, out, rules):
+        stream = torch._C._cuda_getCurrentRawStream(self._device_index)
+        space = self._choice_spaces.get(stream)
+        if space is not None and not torch.cuda.is_current_stream_capturing():
+            chosen = self._direct.mie_direct_choose(*self._choose_entries, self._device_index, logits, rules, temperatures, seeds, counters, out, *space[2:], stream)
+            if chosen is not None:
+                return chosen
         R, V = self._check_logits("sample", logits)
         dev, i32 = self._device_index, torch.int32
         if logits.get_device() != dev:
@@ -2124,34 +2147,35 @@ class HipBackend(KernelBackend):
             out = torch.empty(R, dtype=i32, device=logits.device)
         o = _rules_vector("sample", "out", out, i32, R, dev)
         lib = self.lib("logit_rules")
-        if (R, V) not in self._rule_slices:
-            if len(self._rule_slices) >= 4096:
-                self._rule_slices.clear()
-            self._rule_slices[(R, V)] = lib.mie_rules_slices(R, V)
-        slices, best, arrived = self._rule_slices[(R, V)], 0, 0
-        if slices > 1:
-            if torch.cuda.is_current_stream_capturing():        # a graph may run beside anything: memory of its own, a launch more
-                workspace = torch.empty(R * slices, dtype=torch.int64, device=logits.device)
-                best = workspace.data_ptr()
-            else:
-                best, arrived = self._choice_workspace(R, slices)
+        slices, best, arrived = lib.mie_rules_slices(R, V), 0, 0
+        if not torch.cuda.is_current_stream_capturing():
+            best, arrived = self._choice_workspace(stream, R, slices)
+        elif slices > 1:                                        # a graph may run beside anything: memory of its own, a launch more
+            workspace = torch.empty(R * slices, dtype=torch.int64, device=logits.device)
+            best = workspace.data_ptr()
         library.check(lib, lib.mie_choose_by_rules(
-            logits.data_ptr(), logits.stride(0) if R > 1 else V, *args, t, s, c, best, arrived, o, R, V,
-            self._stream()))
+            logits.data_ptr(), logits.stride(0) if R > 1 else V, *args, t, s, c, best, arrived, o, R, V, c_void_p(stream)))
         return out
 
-    def _choice_workspace(self, R, slices):
+    def _choice_workspace(self, stream, R, slices):
         """Addresses of the candidates of a choice's slices and of the counters by which the last of them is known, of the current
         stream's own: calls on one stream run one after another, and each leaves the counters at 0."""
-        stream = torch._C._cuda_getCurrentRawStream(self._device_index)
-        best, arrived = self._choice_spaces.get(stream, (None, None))
-        if best is None or best.numel() < R * slices or arrived.numel() < 32 * R:
-            best = torch.empty(max(R * slices, 8192), dtype=torch.int64, device=self.device)
-            arrived = torch.zeros(32 * max(R, 256), dtype=torch.int32, device=self.device)
-            self._choice_spaces[stream] = best, arrived
-        return best.data_ptr(), arrived.data_ptr()
+        candidates, rows = self._choice_spaces[stream][4:] if stream in self._choice_spaces else (0, 0)
+        if candidates < R * slices or rows < R or not candidates:
+            candidates, rows = max(R * slices, 8192), max(R, 256)
+            best = torch.empty(candidates, dtype=torch.int64, device=self.device)
+            arrived = torch.zeros(32 * rows, dtype=torch.int32, device=self.device)
+            self._choose_entries = [self._entry(self.lib("logit_rules"), n) for n in ("mie_choose_by_rules", "mie_rules_slices")]
+            self._choice_spaces[stream] = best, arrived, best.data_ptr(), arrived.data_ptr(), candidates, rows
+        return self._choice_spaces[stream][2:4]
 
     def adjust_logits(self, logits, rules, out=None):
+        if self._adjust_entry is None:
+            self._adjust_entry = self._entry(self.lib("logit_rules"), "mie_adjust_logits")
+        adjusted = self._direct.mie_direct_adjust(self._adjust_entry, self._device_index, logits, rules, out,
+                                                  torch._C._cuda_getCurrentRawStream(self._device_index))
+        if adjusted is not None:
+            return adjusted
         R, V = self._check_logits("adjust_logits", logits)
         if logits.get_device() != self._device_index or (out is not None and out.get_device() != self._device_index):
             raise ValueError("adjust_logits: logits and out belong on this GPU")

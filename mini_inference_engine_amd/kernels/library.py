@@ -33,24 +33,26 @@ class KernelModule:
     ctypes argument types (every entry point returns int: 0, or a negative code with a message readable
     through <name>_last_error()).  ``variants``: lists of -D defines built ahead of time; others compile at
     first use.  ``flags``: compiler flags beside FLAGS.  ``source``: the .hip file (by default csrc/<name>.hip);
-    a module outside the package hashes its own file and this package's headers."""
+    a module outside the package hashes its own file and this package's headers.  ``objects``: its entry points
+    take and return Python objects and are called with Python's lock held."""
 
-    def __init__(self, name, signatures=None, variants=None, flags=None, source=None):
+    def __init__(self, name, signatures=None, variants=None, flags=None, source=None, objects=False):
         self.name = name
         self.signatures = dict(signatures or {})
         self.variants = [tuple(v) for v in (variants or [()])]
         self.flags = list(flags or [])
         self.source = source or os.path.join(CSRC, name + ".hip")
+        self.objects = objects
 
 
 MODULES: dict[str, KernelModule] = {}
 
 
-def register_kernel_module(name: str, signatures=None, variants=None, flags=None, source=None) -> KernelModule:
+def register_kernel_module(name: str, signatures=None, variants=None, flags=None, source=None, objects=False) -> KernelModule:
     """Make a kernel source known to the loader, the build-everything step and the backend's
     declaration of argument types.  A part that brings a kernel of its own calls this (from outside the
     package too) and then reaches its entry points through ``HipBackend.lib(name)``."""
-    MODULES[name] = KernelModule(name, signatures, variants, flags, source)
+    MODULES[name] = KernelModule(name, signatures, variants, flags, source, objects)
     return MODULES[name]
 
 
@@ -201,7 +203,7 @@ def load(module: str, defines: tuple = ()) -> ctypes.CDLL:
             return _loaded[key]
         path = find_built(module, tuple(defines)) or build(module, tuple(defines))
         try:
-            lib = ctypes.CDLL(path)
+            lib = (ctypes.PyDLL if kernel_module(module).objects else ctypes.CDLL)(path)
         except OSError as e:
             raise KernelLibraryError(f"cannot load {path}: {e}") from e
         err = getattr(lib, f"{module}_last_error")
@@ -211,7 +213,7 @@ def load(module: str, defines: tuple = ()) -> ctypes.CDLL:
         for entry, argtypes in kernel_module(module).signatures.items():
             fn = getattr(lib, entry)
             fn.argtypes = list(argtypes)
-            fn.restype = ctypes.c_int
+            fn.restype = ctypes.py_object if kernel_module(module).objects else ctypes.c_int
         _loaded[key] = lib
         return lib
 

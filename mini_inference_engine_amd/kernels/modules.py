@@ -1,7 +1,11 @@
 """The package's own kernel modules: source name, entry points with their argument types, the variants
 built ahead of time and extra compiler flags.  Registered with the loader on import; a part that brings a
 kernel of its own registers it the same way (library.register_kernel_module)."""
-from ctypes import c_float, c_int, c_long, c_void_p
+import os
+import sysconfig
+from ctypes import c_double, c_float, c_int, c_long, c_void_p, py_object
+
+import torch
 
 from .library import register_kernel_module
 from .variants import HEAD_DIMS
@@ -175,6 +179,15 @@ register_kernel_module("shared_attention", {
     "mie_shared_attention_head_dim": [],
     "mie_shared_attention": [P, L, P, P, P, I, P, P, P, I, I, P, I, P, I, I, I, P, I, I, I, I, F, F, P, P],
 }, variants=_head_variants, flags=["-mllvm", "-amdgpu-mfma-vgpr-form"])
+# direct_calls: host code only, entry points that take tensors.
+_torch, O = os.path.dirname(torch.__file__), py_object
+register_kernel_module("direct_calls", {
+    "mie_direct_adjust": [P, I, O, O, O, P],
+    "mie_direct_choose": [P, P, I, O, O, O, O, O, O, P, P, L, L, P],
+    "mie_direct_shared": [P, I, O, O, O, O, O, O, P, c_double, c_double, O, P],
+}, flags=[f"-I{_torch}/include", f"-I{_torch}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-DMIE_TORCH_VERSION=\"{torch.__version__}\"",
+          f"-L{_torch}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{_torch}/lib"], objects=True)
 # lt_gemm: host code only, the engine's own way into the library's matrix products (hipBLASLt) with the choice of
 # kernel per shape kept here.
 register_kernel_module("lt_gemm", {

@@ -8,6 +8,8 @@ An item leaves a partial result for each of its columns; a row's partial results
 """
 from __future__ import annotations
 
+from ctypes import addressof, c_long
+
 import numpy as np
 import torch
 
@@ -129,6 +131,14 @@ class SharedPrefixPlan:
         self._data = data
         self.items, self.row_parts = data[:8 * len(items)], data[8 * len(items):]
         self.addresses = self.items.data_ptr(), self.row_parts.data_ptr()
+        self._numbers = (c_long * 13)(*self.addresses, self.num_items, self.whole_items, self.column_tiles, self.most_parts, self.num_parts, self.num_rows,
+                                      self.num_q_heads, self.num_kv_heads, self.head_dim, self.max_context, data.get_device())
+        self.numbers = addressof(self._numbers)     # the same for csrc/direct_calls.hip
+
+    def exceeded_by(self, step) -> bool:
+        """Whether a row of the step has more keys than it was planned for, as far as the host knows them."""
+        ends = step.host.get("row_context") if step.host else None
+        return ends is not None and bool((ends > self.contexts).any())
 
     def used_on(self, stream: int) -> None:
         """The current stream, ``stream`` by handle, is about to read the plan: another than its own waits for it and keeps its memory."""
@@ -139,21 +149,26 @@ class SharedPrefixPlan:
 
     def _worth_it(self, G: int, units: int, float32: bool) -> bool:
         """Whether contexts are cut and shared keys read once, or every row's whole context is left to one workgroup or wave a kv head, with no
-        partial results and no second launch: as long as that takes no longer.  Measured, us, whole / shared by (rows x kv heads) / 256; a
-        caller that launches one call after another adds to the second up to 17, which its two launches take from the host.
-          bfloat16, heads of 64:   1 to 2: 1,500 keys 10 to 14 / 14;   3: 800 keys 17 / 14;   4.3: 400 keys 16 / 15;   8: 400 keys 15 / 19, 800 25 / 21
-          of 128:    1 to 2: 800 keys 11 to 14 / 15 to 17;   3: 400 keys 15 / 17, 800 24 / 20;   4.3: 200 keys 15 / 18, 400 23 / 20;   8: 400 keys 21 / 27, 800 35 / 27
-          of 256:    1 to 2: 400 keys 15 to 20 / 15 to 22;   3: 200 keys 17 / 25, 400 24 / 26;   4.3: 100 keys 22 / 25, 200 32 / 27;   8: 200 keys 35 / 37
-          float32, of 64:   1: 800 keys 17 / 13;   2: 400 keys 16 / 13;   3: 200 keys 16 / 14;   4.3: 100 keys 16 / 14, 200 23 / 18;   8: 200 keys 24 / 27
-          of 128:    1: 200 keys 17 / 14;   2: 100 keys 16 / 16;   3: 30 keys 16 / 20, 100 25 / 18;   4.3: 30 keys 22 / 28;   8: 30 keys 31 / 40, 100 47 / 39
-          one wave takes all keys, 4 heads of 48: 0.1 to 1: 500 keys 12 / 7 to 11, 700 15 to 16 / 7 to 11;   4: 200 keys 14 / 15, 350 18 / 15
-          2 heads of 128 with 20 query heads each: 0.5: 500 keys 15 / 16;   2: 700 keys 22 / 29;   float32: 0.5: 100 keys 15 / 15, 200 23 / 18"""
+        partial results and no second launch: as long as that takes no longer.  Measured, us, whole / shared by (rows x kv heads) / 256.
+          bfloat16, heads of 64:   0.1: 700 keys 8 / 8, 1,500 keys 11 / 8;   0.5 to 2: 1,500 keys 11 to 14 / 13 to 14;   3: 800 keys 17 / 14;   4.3: 400 keys
+          16 / 15;   8: 400 keys 15 / 19, 800 25 / 21
+          of 128:    0.1 to 2: 1,000 keys 12 to 16 / 12 to 17;   3: 400 keys 15 / 17, 800 24 / 20;   4.3: 200 keys 15 / 18, 400 23 / 20;   8: 400 keys 21 / 27, 800
+          35 / 27;   of 256:   0.1 to 2: 500 keys 16 to 24 / 14 to 22;   3: 200 keys 17 / 25, 400 24 / 26;   4.3: 100 keys 22 / 25, 200 32 / 27;   8: 200 keys 35 / 37
+          float32, of 64:   0.1 to 1: 350 keys 10 / 9 to 12, 500 keys 13 / 10 to 14;   2: 200 keys 11 / 11, 400 16 / 13;   3: 100 keys 11 / 13, 200 16 / 14;   4.3: 100 keys
+          16 / 14;   8: 100 keys 16 / 23, 200 24 / 27
+          of 128:    0.1 to 1: 100 keys 11 / 13, 200 17 / 14;   2: 100 keys 16 / 16;   3: 30 keys 16 / 20, 100 25 / 18;   4.3: 30 keys 22 / 28;   8: 30 keys 31 / 40, 100 47 / 39
+          of 256:    0.1 to 1: 100 keys 19 / 21, 200 30 / 21;   4: 100 keys 60 / 45
+          one wave takes all keys, heads of 48 and 80:   0.1: 200 keys 8 / 7;   0.5 to 1: 350 keys 10 / 11 to 12, 500 12 to 13 / 11;   4: 200 keys 13 / 15, 350 17 / 15
+          heads of 128 with 20 query heads each:   0.1: 350 keys 11 / 13, 500 14 / 12;   0.5: 500 keys 15 / 16, 700 18 / 17;   2: 700 keys 22 / 29;   float32:  0.1
+          to 0.5: 100 keys 15 / 13 to 15;   2: 200 keys 35 / 36"""
         D, load = self.head_dim, self.num_rows * self.num_kv_heads / units
         sharers = _sharers(D, float32)
-        if G > 16 or not sharers:
-            most, rounds = 16384 // D if float32 else min(640, 81920 // D), load / 2
+        if G > 16:
+            most, rounds = (10000 // D * max(1, load), 1) if float32 else (min(640, 81920 // D), load / 3)
+        elif not sharers:
+            most, rounds = 420, load / 2
         elif float32:
-            most, rounds = 14400 * sharers // D, min(load, max(4, load / 2))
+            most, rounds = (28800 // D, max(min(load, 4), load / 4)) if sharers == 4 else (max(112, 17000 // D), max(min(load, 2.5), load / 4))
         else:
-            most, rounds = min(1536, 131072 // D), -(-load // 2) if load <= 6 else 0.3 * load
+            most, rounds = min(1536 if load >= 0.5 else 900, 131072 // D), -(-load // 2) if load <= 6 else 0.3 * load
         return self.max_context * max(1, rounds) > most

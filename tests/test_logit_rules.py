@@ -3,7 +3,9 @@
 Tolerance: a logit passes at most five operations of 32 bits (division or product, product, two subtractions, addition), each off by
 at most 2^-24 of its result; with |z| the largest magnitude met on the way the sum of the errors is at most 5 * 2^-24 * |z|.
 """
+import dataclasses
 import math
+import sys
 
 import pytest
 import torch
@@ -388,3 +390,98 @@ def test_a_captured_choice_beside_calls(ops):
             here = [ops.sample(inputs[2], temps, seeds, counters, rules=rules) for _ in range(3)]
         torch.cuda.synchronize()
         assert torch.equal(outs[0], wants[0]) and torch.equal(outs[1], wants[1]) and all(torch.equal(h, wants[2]) for h in here)
+
+
+class TheLongWay:
+    """Declines every call, as the short way declines what it does not take."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.fixture
+def long_ops(ops):
+    ops.adjust_logits(torch.zeros((1, 8), device="cuda"), LogitRules())          # (the short way is there)
+    short, ops._direct = ops._direct, TheLongWay()
+    yield ops
+    ops._direct = short
+
+
+def calls(ops, size, out):
+    R, V, history = size
+    rules = make(R, V, history, 11, "cuda")
+    g = torch.Generator().manual_seed(4)
+    logits = 4 * torch.randn((R, V + 5), generator=g).cuda()[:, :V]
+    temps, seeds, counters = torch.rand(R, generator=g).cuda(), torch.arange(R).cuda() * 7919, torch.arange(R, dtype=torch.int32).cuda()
+    made = []
+    for _ in range(2):                              # (the first choice on a stream makes its workspace, and goes the long way)
+        chosen = torch.full((R,), -5, dtype=torch.int32, device="cuda") if out else None
+        adjusted = torch.full((R, V + 3), 9.0, device="cuda")[:, :V] if out else None
+        made += [ops.sample(logits, temps, seeds, counters, out=chosen, rules=rules), ops.adjust_logits(logits, rules, out=adjusted)]
+        assert not out or (made[-2] is chosen and made[-1] is adjusted)
+    return made
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [False, True])
+@pytest.mark.parametrize("size", SIZES[:9])
+def test_both_ways_into_the_kernels(ops, size, out):
+    made = calls(ops, size, out)
+    short, ops._direct = ops._direct, TheLongWay()
+    try:
+        for a, b in zip(made, calls(ops, size, out)):
+            assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a.view(torch.int32), b.view(torch.int32))
+    finally:
+        ops._direct = short
+
+
+@pytest.mark.gpu
+def test_a_call_keeps_nothing(ops):
+    """References to what a call was given are as before, taken or declined, and so is the memory."""
+    R, V = 5, 20001
+    rules = make(R, V, 40, 3, "cuda")
+    logits, out = torch.randn((R, V), device="cuda"), torch.empty((R, V), device="cuda")
+    temps, seeds, counters = torch.ones(R, device="cuda"), torch.arange(R).cuda(), torch.zeros(R, dtype=torch.int32, device="cuda")
+    held = [logits, out, temps, seeds, counters, rules, rules.history, rules.slots, rules.masks, rules.bias_values, None]
+
+    def some():
+        for _ in range(50):
+            ops.sample(logits, temps, seeds, counters, rules=rules)
+            ops.adjust_logits(logits, rules, out=out)
+            ops.adjust_logits(logits, rules)
+            for bad in (dict(seeds=counters), dict(logits=logits.double()), dict(temperatures=None), dict(rules=None)):
+                kw = {**dict(logits=logits, temperatures=temps, seeds=seeds, counters=counters, rules=rules), **bad}
+                if kw["rules"] is None:
+                    with pytest.raises(AttributeError):
+                        ops.adjust_logits(logits, None)
+                else:
+                    with pytest.raises(ValueError):
+                        ops.sample(**kw)
+
+    some()
+    torch.cuda.synchronize()
+    before, memory = [sys.getrefcount(x) for x in held[:-1]], torch.cuda.memory_allocated()
+    some()
+    torch.cuda.synchronize()
+    assert [sys.getrefcount(x) for x in held[:-1]] == before and torch.cuda.memory_allocated() == memory
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("short", [True, False])
+@pytest.mark.parametrize("name, change", [
+    ("slots", lambda t: t.long()), ("lengths", lambda t: t[:-1]), ("prompt_lengths", lambda t: t.cpu()), ("repetition", lambda t: t.double()),
+    ("presence", lambda t: torch.stack([t, t], 1)[:, 0]), ("frequency", lambda t: None), ("history", lambda t: t.long()), ("history", lambda t: t[0]),
+    ("history", lambda t: t[:1].expand(3, -1)), ("bias_starts", lambda t: t[:-1]), ("bias_tokens", lambda t: t[:-1]), ("bias_values", lambda t: t.half()),
+    ("masks", lambda t: t[:, :-2]), ("masks", lambda t: t.cpu()), ("mask_rows", lambda t: t[None])])
+def test_refusals_of_both_ways(ops, long_ops, name, change, short):
+    R, V = 4, 10007
+    rules = make(R, V, 40, 3, "cuda")
+    logits = torch.randn((R, V), device="cuda")
+    small = torch.ones(R, device="cuda"), torch.arange(R).cuda(), torch.zeros(R, dtype=torch.int32, device="cuda")
+    if short:
+        ops._direct = ops.lib("direct_calls")
+    ops.sample(logits, *small, rules=rules)
+    bad = dataclasses.replace(rules, **{name: change(getattr(rules, name))})
+    for call in (lambda: ops.sample(logits, *small, rules=bad), lambda: ops.adjust_logits(logits, bad)):
+        with pytest.raises(ValueError, match="bias_values" if name == "bias_tokens" else name):      # (as many values as tokens)
+            call()

@@ -7,6 +7,7 @@ Numerator and denominator both carry that: 2 (e + N 2^-24) A.  In bfloat16 the p
 (2^-8 |out|).
 """
 import math
+import sys
 from types import SimpleNamespace
 
 import numpy as np
@@ -331,6 +332,51 @@ def test_table_entries_that_are_no_page(ops, heads, dtype):
         s.tables[r, p // 16 + 1:] = torch.tensor([-1, 2**31 - 1, -2**31, s.k.shape[0]], dtype=torch.int32).repeat(9)[:s.tables.shape[1] - p // 16 - 1].cuda()
     run(ops, s, groups, *heads, dtype)
     run(ops, s, groups, *heads, dtype, contexts=[200] * 7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (20, 1, 48), (4, 2, 256)])
+@pytest.mark.parametrize("sink", [None, 0.5, "heads"])
+def test_both_ways_into_the_kernels(ops, sink, heads, dtype):
+    """The call that takes the tensors themselves and the one of plain numbers: the same results, the same refusals, nothing kept."""
+    o = ops[dtype]
+    groups = [(6, 100), (3, 0), (30, 48)]
+    s = make(groups, rows_behind(groups, 60, 2), *heads, 16, dtype, extra_stride=8)
+    step, group = step_of(s)
+    contexts = [p + 1 for p in s.positions.tolist()]
+    sink = torch.linspace(-1, 1, heads[0], device="cuda") if sink == "heads" else sink
+    plans = [o.plan_shared_prefix(groups, contexts, *heads, share=share) for share in (True, False)]
+
+    def call(**kw):
+        a = {**dict(q=s.q, k=s.k, v=s.v, group=group, step=step, scale=0.2, plan=plans[0], sink=sink), **kw}
+        return o.shared_prefix_attention(a["q"], *heads, a["k"], a["v"], a["group"], a["step"], a["scale"], a["plan"], sink=a["sink"])
+
+    def refusals():
+        for bad in (dict(q=s.q.double()), dict(q=s.q[:, :heads[0] * heads[2] - 1]), dict(q=s.q.t()), dict(k=s.k[:, :, :8]), dict(v=s.v.transpose(2, 3)),
+                    dict(k=s.k.cpu()), dict(plan=SharedPrefixPlan(groups, contexts, *heads, "cpu", float32=dtype == F32)), dict(plan=None), dict(scale=math.inf),
+                    dict(scale=0.0), dict(group=SimpleNamespace(block_tables=s.tables[:5])), dict(group=SimpleNamespace(block_tables=s.tables[:, :-1])),
+                    dict(step=step_of(s, num_rows=4)[0]), dict(step=step_of(s, token_row=step.token_row[:-1])[0]), dict(step=step_of(s, most=10 ** 6)[0]),
+                    dict(step=step_of(s, positions=step.positions.long())[0]), dict(sink=torch.zeros(heads[0] + 1, device="cuda"))):
+            with pytest.raises((ValueError, TypeError)):
+                call(**bad)
+
+    call()
+    short = [call(plan=p) for p in plans]
+    held = [s.q, s.k, s.v, s.tables, step.positions, step.token_row, plans[0], plans[1]._data]
+    before, memory = [sys.getrefcount(x) for x in held], torch.cuda.memory_allocated()
+    for _ in range(20):
+        call()
+    refusals()
+    assert [sys.getrefcount(x) for x in held] == before and torch.cuda.memory_allocated() == memory
+    direct, o._direct = o._direct, SimpleNamespace(mie_direct_shared=lambda *args: None)
+    try:
+        refusals()
+        for a, p in zip(short, plans):
+            b = call(plan=p)
+            assert a.dtype == b.dtype and torch.equal(a, b)
+    finally:
+        o._direct = direct
 
 
 @pytest.mark.gpu
