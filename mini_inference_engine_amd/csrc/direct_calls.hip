@@ -1,6 +1,7 @@
 // The short way from Python into kernels that a step calls with many small tensors: one call takes the tensors themselves, sees that
-// they are as the kernel needs them, makes what it returns and launches.  Host code only.  (The same from Python, tensor by tensor, with
-// an entry point of plain numbers: choosing under rules 15.6 us a call, adjusting 13.7, attention over shared keys 11.5, of which a launch is 3.)
+// they are as the kernel needs them, makes what it returns and launches.  Host code only.  (A call of the smallest sizes, us, from Python tensor
+// by tensor with an entry point of plain numbers, and this way: choosing under rules 15.7 and 7.2, adjusting 13.9 and 5.6, attention over shared
+// keys 11.7 and 6.1; a launch is 3 of each.)
 //
 // Every entry point returns a tensor, or None where something is not as it has to be or is none of the usual cases: the caller then goes
 // the long way, which says what is wrong.  Loaded with Python's lock held throughout.
