@@ -13,12 +13,13 @@
 // the slice's logits, asked for before the text is read, past those words.  Every slice reads the row's whole text; it comes from the L2 for
 // all slices but one.  Biases are settled after that, the last of a token's entries first.
 //
-// What bounds it, of what a call cannot do without (MI355X): 256 rows of 128,256 with texts of 700 to 2,000 tokens chosen in 54 us, where
+// What bounds it, of what a call cannot do without (MI355X): 256 rows of 128,256 with texts of 700 to 2,000 tokens chosen in 52 us, where
 // the 134 MB of logits take 26 at the rate of a large copy: reading alone, in this division, takes 34 with the join of the slices, texts 8, biases 6, masks 4,
 // noise on a quarter of the rows 5, and half of the waves' time is waiting for the four dependent loads that a workgroup begins with.
-// 192 rows with texts of 4,000 to 12,000 adjusted in 55 us, 40 for their 205 MB: reading every text 32 times is two fifths of the
-// instructions.  Tried and slower: slices of 8,192 on 512 threads (62 and 59 us); tokens with a word gathered in a list and taken by themselves (64
-// and 57); a bound on the noise by one logarithm before the exact two (63); text and list asked for before the words are cleared (62 and 79).
+// 192 rows with texts of 4,000 to 12,000 adjusted in 53 us, 40 for their 205 MB: reading every text 32 times is two fifths of the
+// instructions.  Tried and slower (us of the two): slices of 8,192 on 512 threads (62 and 59) or on 256 (62 and 59), of 6,144 (52.5 and 53); tokens
+// with a word gathered in a list and taken by themselves (64 and 57); a bound on the noise by one logarithm before the exact two (63); text and
+// list asked for before the words are cleared (62 and 79).
 #include "launch.hpp"
 #include "sampling.hpp"
 #include <type_traits>
