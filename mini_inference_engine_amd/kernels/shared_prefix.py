@@ -135,6 +135,12 @@ class SharedPrefixPlan:
                                       self.num_q_heads, self.num_kv_heads, self.head_dim, self.max_context, data.get_device())
         self.numbers = addressof(self._numbers)     # the same for csrc/direct_calls.hip
 
+    def __deepcopy__(self, memo):
+        return self                                 # nothing of a plan changes, and the addresses are of its own memory
+
+    def __reduce__(self):
+        raise TypeError("a plan is addresses of this process's memory")
+
     def exceeded_by(self, step) -> bool:
         """Whether a row of the step has more keys than it was planned for, as far as the host knows them."""
         ends = step.host.get("row_context") if step.host else None

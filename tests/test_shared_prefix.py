@@ -6,7 +6,9 @@ sum |q k|, and 2^-21 for the exponential, its argument's rounding (|x| up to 64)
 Numerator and denominator both carry that: 2 (e + N 2^-24) A.  In bfloat16 the p of the numerator are rounded (2^-8 A) and the result is
 (2^-8 |out|).
 """
+import copy
 import math
+import pickle
 import sys
 from types import SimpleNamespace
 
@@ -452,6 +454,15 @@ def test_a_plan_covers_every_key_once(seed, share):
     shared = any(columns > G for _, columns, *_ in plan.items.view(-1, 8).tolist())
     if share is not None:
         assert shared == (share and any(n > 1 and k > 0 for n, k in groups))
+
+
+def test_a_plan_is_not_copied():
+    plan = SharedPrefixPlan([(2, 5)], [6, 7], 4, 2, 64, "cpu")
+    assert copy.deepcopy(plan) is plan
+    with pytest.raises(TypeError, match="plan"):
+        pickle.dumps(plan)
+    with pytest.raises(TypeError, match="plan"):
+        copy.copy(plan)
 
 
 @pytest.mark.parametrize("bad", [([(2, 5)], [5, 4], 4, 2), ([(2, 5)], [5], 4, 2), ([(0, 5), (1, 0)], [5], 4, 2), ([(1, -1)], [5], 4, 2),
