@@ -78,6 +78,30 @@ __device__ __forceinline__ unsigned long long pack_candidate(float v, int i) {
   return ((unsigned long long)__float_as_uint(v) << 32) | (uint32_t)i;
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int from_lane(int x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, ROWS, 0xF, false); }
+
+// The largest (or smallest) of a wave's 64 numbers, for every lane.
+template <bool LARGEST>
+__device__ __forceinline__ int wave_extreme(int x) {
+  auto pick = [](int a, int b) { return LARGEST ? (a > b ? a : b) : (a < b ? a : b); };
+  x = pick(x, from_lane<0x111, 0xF>(x));       // from 1, 2, 4 and 8 lanes before in a row of 16, then from the last lane of the row and the half before
+  x = pick(x, from_lane<0x112, 0xF>(x));
+  x = pick(x, from_lane<0x114, 0xF>(x));
+  x = pick(x, from_lane<0x118, 0xF>(x));
+  x = pick(x, from_lane<0x142, 0xA>(x));
+  x = pick(x, from_lane<0x143, 0xC>(x));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The best of a wave's candidates, for every lane: floats (none NaN) in order as integers (-0 as 0), then the lowest index of the largest.
+__device__ __forceinline__ void wave_best(float& bv, int& bi) {
+  auto turn = [](int bits) { return bits ^ (bits >> 31 & 0x7FFFFFFF); };
+  const int mine = turn(__float_as_int(bv + 0.f)), most = wave_extreme<true>(mine);
+  bi = wave_extreme<false>(mine == most ? bi : 0x7FFFFFFF);
+  bv = __int_as_float(turn(most));
+}
+
 // The token of the best of n candidates, for every lane of a wave.
 __device__ __forceinline__ int best_of_row(const unsigned long long* best, int n) {
   float bv = -INFINITY;
@@ -86,16 +110,11 @@ __device__ __forceinline__ int best_of_row(const unsigned long long* best, int n
     const unsigned long long c = __hip_atomic_load(&best[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     sample_better(__uint_as_float((uint32_t)(c >> 32)), (int)(uint32_t)c, bv, bi);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ov = __shfl_xor(bv, o, 64);
-    const int oi = __shfl_xor(bi, o, 64);
-    sample_better(ov, oi, bv, bi);
-  }
+  wave_best(bv, bi);
   return bi == 0x7FFFFFFF ? 0 : bi;
 }
 
-// Grid (workgroups a row, rows); a workgroup takes every gridDim.x-th slice.  CHOOSE: its best candidate to best [rows, workgroups], or,
+// Grid (slices of a row, rows), a workgroup each.  CHOOSE: its best candidate to best [rows, workgroups], or,
 // of a row that has one workgroup, the token to ``chosen``; else the adjusted logits to ``out``.  With ``arrived`` (a counter a
 // row, 0 before and after) the last workgroup of a row to arrive joins the row's candidates: one launch instead of two.
 template <bool CHOOSE, int THREADS>
@@ -136,113 +155,116 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
   float bv = -INFINITY;
   int bi = 0x7FFFFFFF;
   const bool counted = length > 0 || listed > 0;                      // (the same in the whole workgroup)
-  for (int begin = blockIdx.x * slice; begin < V; begin += gridDim.x * slice) {
-    const int n = min(slice, V - begin), n4 = n & ~3;
-    const float* z0 = logits + (size_t)r * ld + begin;
-    // the slice's logits and mask are asked for before the text is read
-    f32x4_any z[AHEAD];
-    uint32_t bits[AHEAD];
+  const int begin = blockIdx.x * slice;
+  const int n = min(slice, V - begin), n4 = n & ~3;
+  const float* z0 = logits + (size_t)r * ld + begin;
+  // The list's first entries, one a thread, then the slice's logits and mask are asked for before the text is read.
+  const unsigned own = tid < listed ? (unsigned)list[tid] - (unsigned)begin : ~0u;
+  const float own_value = tid < listed ? list_values[tid] : 0.f;
+  f32x4_any z[AHEAD];
+  uint32_t bits[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int i = (k * THREADS + tid) * 4;
-      if (i < n4) {
-        z[k] = *reinterpret_cast<const f32x4_any*>(z0 + i);
-        bits[k] = mask ? mask[(begin + i) >> 5] >> ((begin + i) & 31) : 15u;
+  for (int k = AHEAD - 1; k >= 0; --k) {
+    const int i = (k * THREADS + tid) * 4;
+    if (i < n4) {
+      z[k] = *reinterpret_cast<const f32x4_any*>(z0 + i);
+      bits[k] = mask ? mask[(begin + i) >> 5] >> ((begin + i) & 31) : 15u;
+    }
+  }
+  if (counted) {
+    const int zeros = (n + 3) / 4;
+    for (int i = tid; i < zeros; i += THREADS) {
+      reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    auto count = [&](int token, int i) {
+      const unsigned at = (unsigned)token - (unsigned)begin;        // what is no token of the vocabulary is in no slice
+      if (at < (unsigned)n) {
+        atomicOr(&words[at], SEEN);
+        if (i >= prompt) atomicAdd(&words[at], 1u);
+      }
+    };
+    const int length4 = length & ~3;
+    constexpr int READS = 4;                                        // on their way together
+    for (int i0 = tid * 4; i0 < length4; i0 += READS * THREADS * 4) {
+      i32x4_any t[READS];
+#pragma unroll
+      for (int k = 0; k < READS; ++k) {
+        const int i = i0 + k * THREADS * 4;
+        t[k] = *reinterpret_cast<const i32x4_any*>(text + (i < length4 ? i : i0));
+      }
+#pragma unroll
+      for (int k = 0; k < READS; ++k) {
+        const int i = i0 + k * THREADS * 4;
+        if (i >= length4) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) count(t[k][j], i + j);
       }
     }
-    if (counted) {
-      if (begin != (int)blockIdx.x * slice) __syncthreads();          // the words of the slice before have been read
-      const int zeros = (n + 3) / 4;
-      for (int i = tid; i < zeros; i += THREADS) {
-        reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
-      }
-      __syncthreads();
-      auto count = [&](int token, int i) {
-        const unsigned at = (unsigned)token - (unsigned)begin;        // what is no token of the vocabulary is in no slice
-        if (at < (unsigned)n) {
-          atomicOr(&words[at], SEEN);
-          if (i >= prompt) atomicAdd(&words[at], 1u);
-        }
-      };
-      const int length4 = length & ~3;
-      constexpr int READS = CHOOSE ? 2 : 4;                           // on their way together
-      for (int i0 = tid * 4; i0 < length4; i0 += READS * THREADS * 4) {
-        i32x4_any t[READS];
-#pragma unroll
-        for (int k = 0; k < READS; ++k) {
-          const int i = i0 + k * THREADS * 4;
-          t[k] = *reinterpret_cast<const i32x4_any*>(text + (i < length4 ? i : i0));
-        }
-#pragma unroll
-        for (int k = 0; k < READS; ++k) {
-          const int i = i0 + k * THREADS * 4;
-          if (i >= length4) break;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) count(t[k][j], i + j);
-        }
-      }
-      if (length4 + tid < length) count(text[length4 + tid], length4 + tid);
-      for (int i = tid; i < listed; i += THREADS) {
-        const unsigned at = (unsigned)list[i] - (unsigned)begin;
-        if (at < (unsigned)n) atomicOr(&words[at], BIASED);
-      }
-      __syncthreads();
+    if (length4 + tid < length) count(text[length4 + tid], length4 + tid);
+    if (own < (unsigned)n) atomicOr(&words[own], BIASED);
+    for (int i = tid + THREADS; i < listed; i += THREADS) {
+      const unsigned at = (unsigned)list[i] - (unsigned)begin;
+      if (at < (unsigned)n) atomicOr(&words[at], BIASED);
     }
-    float* o0 = CHOOSE ? nullptr : out + (size_t)r * out_ld + begin;
+    __syncthreads();
+  }
+  float* o0 = CHOOSE ? nullptr : out + (size_t)r * out_ld + begin;
+  // A thread goes through its tokens from the last to the first, so that one comparison keeps the first of equals (and no NaN).
+  auto keep = [&](float y, int i) {
+    const float v = sample_value(y, begin + i, noisy, inv_t, key);
+    const bool better = v >= bv;
+    bv = better ? v : bv;
+    bi = better ? begin + i : bi;
+  };
+  if (n4 + tid < n) {                                               // up to three at the end of the row
+    const int i = n4 + tid;
+    const uint32_t w = counted ? words[i] : 0;
+    const bool may = !mask || (mask[(begin + i) >> 5] >> ((begin + i) & 31) & 1);
+    const float z1 = z0[i], y = w & BIASED ? z1 : may ? apply_rules(z1, w, row) : -INFINITY;
+    if (!CHOOSE) o0[i] = y;
+    else if (!(w & BIASED)) keep(y, i);
+  }
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int i = (k * THREADS + tid) * 4;
-      if (i >= n4) break;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (counted) w = *reinterpret_cast<const uint4*>(words + i);
+  for (int k = AHEAD - 1; k >= 0; --k) {
+    const int i = (k * THREADS + tid) * 4;
+    if (i >= n4) continue;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (counted) w = *reinterpret_cast<const uint4*>(words + i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t wj = j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
-        const float y = bits[k] >> j & 1 ? apply_rules(z[k][j], wj, row) : -INFINITY;
-        if (wj & BIASED) continue;                                    // left as it is to the list, below
-        if (CHOOSE) sample_consider(y, begin + i + j, noisy, inv_t, key, bv, bi);
-        else z[k][j] = y;
-      }
-      if (!CHOOSE) *reinterpret_cast<f32x4_any*>(o0 + i) = z[k];
+    for (int j = 3; j >= 0; --j) {
+      const uint32_t wj = j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
+      const float y = bits[k] >> j & 1 ? apply_rules(z[k][j], wj, row) : -INFINITY;
+      if (wj & BIASED) continue;                                    // left as it is to the list, below
+      if (CHOOSE) keep(y, i + j);
+      else z[k][j] = y;
     }
-    if (n4 + tid < n) {                                               // up to three at the end of the row
-      const int i = n4 + tid;
-      const uint32_t w = counted ? words[i] : 0;
-      const bool may = !mask || (mask[(begin + i) >> 5] >> ((begin + i) & 31) & 1);
-      const float z1 = z0[i], y = w & BIASED ? z1 : may ? apply_rules(z1, w, row) : -INFINITY;
-      if (!CHOOSE) o0[i] = y;
-      else if (!(w & BIASED)) sample_consider(y, begin + i, noisy, inv_t, key, bv, bi);
-    }
-    // The tokens with a bias, a thread an entry of the list, the list's end first.  Of several entries of a token the last one
-    // has it: within a round the largest thread that asks for it, and what a round has settled has lost its mark for those before.
-    for (int i0 = (listed - 1) / THREADS * THREADS; listed > 0 && i0 >= 0; i0 -= THREADS) {
-      const int e = i0 + tid;
-      const unsigned at = e < listed ? (unsigned)list[e] - (unsigned)begin : ~0u;
-      const bool mine = at < (unsigned)n;
-      __syncthreads();                                                // (and the logits as they were are in memory)
-      const uint32_t w = mine ? words[at] : 0;
-      const bool asks = w & BIASED;
-      __syncthreads();
-      if (asks) words[at] = 0;
-      __syncthreads();
-      if (asks) atomicMax(&words[at], (uint32_t)tid + 1);
-      __syncthreads();
-      if (asks && words[at] == (uint32_t)tid + 1) {
-        const int v = begin + (int)at;
-        const bool may = !mask || (mask[v >> 5] >> (v & 31) & 1);
-        const float y = may ? apply_rules(z0[at], w & ~BIASED, row) + list_values[e] : -INFINITY;
-        if (CHOOSE) sample_consider(y, v, noisy, inv_t, key, bv, bi);
-        else o0[at] = y;
-      }
+    if (!CHOOSE) *reinterpret_cast<f32x4_any*>(o0 + i) = z[k];
+  }
+  // The tokens with a bias, a thread an entry of the list, the list's end first.  Of several entries of a token the last one
+  // has it: within a round the largest thread that asks for it, and what a round has settled has lost its mark for those before.
+  for (int i0 = (listed - 1) / THREADS * THREADS; listed > 0 && i0 >= 0; i0 -= THREADS) {
+    const int e = i0 + tid;
+    const unsigned at = i0 == 0 ? own : e < listed ? (unsigned)list[e] - (unsigned)begin : ~0u;
+    const bool mine = at < (unsigned)n;
+    __syncthreads();                                                // (and the logits as they were are in memory)
+    const uint32_t w = mine ? words[at] : 0;
+    const bool asks = w & BIASED;
+    __syncthreads();
+    if (asks) words[at] = 0;
+    __syncthreads();
+    if (asks) atomicMax(&words[at], (uint32_t)tid + 1);
+    __syncthreads();
+    if (asks && words[at] == (uint32_t)tid + 1) {
+      const int v = begin + (int)at;
+      const bool may = !mask || (mask[v >> 5] >> (v & 31) & 1);
+      const float y = may ? apply_rules(z0[at], w & ~BIASED, row) + (i0 == 0 ? own_value : list_values[e]) : -INFINITY;
+      if (CHOOSE) sample_consider(y, v, noisy, inv_t, key, bv, bi);
+      else o0[at] = y;
     }
   }
   if (!CHOOSE) return;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ov = __shfl_xor(bv, o, 64);
-    const int oi = __shfl_xor(bi, o, 64);
-    sample_better(ov, oi, bv, bi);
-  }
+  wave_best(bv, bi);
   if ((tid & 63) == 0) { wave_v[tid >> 6] = bv; wave_i[tid >> 6] = bi; }
   __syncthreads();
   if (tid >= 64) return;

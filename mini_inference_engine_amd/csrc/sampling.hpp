@@ -12,13 +12,19 @@ __device__ __forceinline__ uint32_t fmix32(uint32_t x) {
   return x;
 }
 
-// One candidate: its value after temperature and noise, kept if it beats the best so far.
-__device__ __forceinline__ void sample_consider(float z, int v, bool noisy, float inv_t, uint32_t key, float& bv, int& bi) {
+// A candidate's value after temperature and noise.
+__device__ __forceinline__ float sample_value(float z, int v, bool noisy, float inv_t, uint32_t key) {
   if (noisy) {
     const uint32_t x = fmix32(key ^ fmix32((uint32_t)v + 0x9E3779B9u));
     const float u = ((float)(x >> 9) + 0.5f) * 1.1920928955078125e-07f;   // 2^-23
     z = fmaf(z, inv_t, -logf(-logf(u)));
   }
+  return z;
+}
+
+// One candidate, kept if it beats the best so far.
+__device__ __forceinline__ void sample_consider(float z, int v, bool noisy, float inv_t, uint32_t key, float& bv, int& bi) {
+  z = sample_value(z, v, noisy, inv_t, key);
   if (z > bv || (z == bv && v < bi)) { bv = z; bi = v; }
 }
 

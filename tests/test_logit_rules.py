@@ -485,3 +485,42 @@ def test_refusals_of_both_ways(ops, long_ops, name, change, short):
     for call in (lambda: ops.sample(logits, *small, rules=bad), lambda: ops.adjust_logits(logits, bad)):
         with pytest.raises(ValueError, match="bias_values" if name == "bias_tokens" else name):      # (as many values as tokens)
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 70, 4099, 8192, 20001, 33000])
+@pytest.mark.parametrize("hot", [0.0, 0.7])
+def test_equals_and_rows_without_numbers(ops, V, hot):
+    """The lowest index among equals, wherever its thread, wave or slice; of a row of -infinity and NaN the first -infinity; of NaN alone 0."""
+    g = torch.Generator().manual_seed(V)
+    R = 12
+    logits = torch.randint(-2, 3, (R, V), generator=g).float()
+    logits[1] = torch.where(torch.rand(V, generator=g) < 0.5, 0.0, -0.0)
+    logits[2] = -math.inf
+    logits[3], logits[4] = math.nan, math.nan
+    logits[4, V * 2 // 3:] = -math.inf
+    logits[5, :V - 1] = math.nan
+    logits[6] = 1.0
+    logits[7, ::2] = math.inf
+    logits[8] = 3.0
+    rules = make(R, V, 60, 3, "cuda", masked=False)
+    for name, value in (("repetition", 1.0), ("presence", 0.0), ("frequency", 0.0)):
+        getattr(rules, name)[:9] = value            # (the others' penalties and biases are whole numbers: equals remain)
+        getattr(rules, name)[9:] = {"repetition": 2.0, "presence": 1.0, "frequency": 1.0}[name]
+    rules.bias_values = rules.bias_values.round()
+    starts = rules.bias_starts.clone()
+    starts[:6] = 0
+    rules.bias_starts = starts
+    masks = torch.full((2, (V + 31) // 32), -1, dtype=torch.int32, device="cuda")
+    masks[1] = 0
+    masks[1, -1] = 1
+    rules.masks, rules.mask_rows = masks, torch.tensor([-1, -1, -1, -1, -1, -1, 0, 0, 1, 0, -1, -1], dtype=torch.int32, device="cuda")
+    logits = logits.cuda()
+    small = torch.full((R,), hot, device="cuda"), torch.arange(R).cuda() * 31, torch.arange(R, dtype=torch.int32).cuda()
+    got = ops.sample(logits, *small, rules=rules)
+    adjusted = ops.adjust_logits(logits, rules)
+    assert torch.equal(got, ops.sample(adjusted, *small))
+    if hot == 0:
+        z = adjusted.cpu().nan_to_num(nan=-math.inf, neginf=-1e38)          # (-infinity above NaN)
+        want = [int((row == row.max()).nonzero()[0]) if not torch.isnan(a).all() else 0 for row, a in zip(z, adjusted.cpu())]
+        assert got.tolist() == want
