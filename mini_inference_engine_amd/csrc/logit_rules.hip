@@ -13,13 +13,14 @@
 // the slice's logits, asked for before the text is read, past those words.  Every slice reads the row's whole text; it comes from the L2 for
 // all slices but one.  Biases are settled after that, the last of a token's entries first.
 //
-// What bounds it, of what a call cannot do without (MI355X): 256 rows of 128,256 with texts of 700 to 2,000 tokens chosen in 52 us, where
-// the 134 MB of logits take 26 at the rate of a large copy: reading alone, in this division, takes 34 with the join of the slices, texts 8, biases 6, masks 4,
-// noise on a quarter of the rows 5, and half of the waves' time is waiting for the four dependent loads that a workgroup begins with.
-// 192 rows with texts of 4,000 to 12,000 adjusted in 53 us, 40 for their 205 MB: reading every text 32 times is two fifths of the
-// instructions.  Tried and slower (us of the two): slices of 8,192 on 512 threads (62 and 59) or on 256 (62 and 59), of 6,144 (52.5 and 53); tokens
-// with a word gathered in a list and taken by themselves (64 and 57); a bound on the noise by one logarithm before the exact two (63); text and
-// list asked for before the words are cleared (62 and 79).
+// What bounds it, of what a call cannot do without (MI355X): 256 rows of 128,256 with texts of 700 to 2,000 tokens chosen in 43 us, where the 134 MB
+// of logits take 26 at the rate of a large copy: reading alone, in this division, takes 25 with the join of the slices, texts 7.5, biases 5, masks 1 and
+// noise on a quarter of the rows 6, all of them vector instructions, which keep the units busy for 65 % of the time.  192 rows with texts of 4,000 to
+// 12,000 adjusted in 41 us, 40 for their 205 MB; results are stored past the L2s, where they would push out what the slices share (49 us otherwise;
+// logits read that way: 46.5, and choosing 44.5).  Tried and slower (us of the two, where the present form took 52 and 53): slices of 8,192 on 512
+// threads (62 and 59) or on 256 (62 and 59), of 6,144 (52.5 and 53); tokens with a word gathered in a list and taken by themselves (64 and 57); a bound
+// on the noise by one logarithm before the exact two (63); text and list asked for before the words are cleared (62 and 79).  An entry of the list that
+// claims its token before the text is counted saves three barriers and 1 %.
 #include "launch.hpp"
 #include "sampling.hpp"
 #include <type_traits>
@@ -239,7 +240,7 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
       if (CHOOSE) keep(y, i + j);
       else z[k][j] = y;
     }
-    if (!CHOOSE) *reinterpret_cast<f32x4_any*>(o0 + i) = z[k];
+    if (!CHOOSE) __builtin_nontemporal_store(z[k], reinterpret_cast<f32x4_any*>(o0 + i));
   }
   // The tokens with a bias, a thread an entry of the list, the list's end first.  Of several entries of a token the last one
   // has it: within a round the largest thread that asks for it, and what a round has settled has lost its mark for those before.
@@ -247,7 +248,8 @@ rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float*
     const int e = i0 + tid;
     const unsigned at = i0 == 0 ? own : e < listed ? (unsigned)list[e] - (unsigned)begin : ~0u;
     const bool mine = at < (unsigned)n;
-    __syncthreads();                                                // (and the logits as they were are in memory)
+    if (!CHOOSE) MIE_VMCNT(0);                                      // the logits as they were are in memory
+    __syncthreads();
     const uint32_t w = mine ? words[at] : 0;
     const bool asks = w & BIASED;
     __syncthreads();
