@@ -26,12 +26,10 @@
 #include <type_traits>
 #pragma clang fp contract(off)      // the formulas' roundings, one by one
 
-// Two ways of dividing a row: slices of up to 4,096 tokens on workgroups of 256 threads, and a row that is short in one slice on a
-// workgroup of 1,024 threads.
-constexpr int PART_THREADS = 256, ROW_THREADS = 1024;
+constexpr int THREADS = 256;
 constexpr int AHEAD = 4;                               // reads of four logits a thread, all on their way at once
 constexpr int ARRIVED = 32;                            // numbers from one row's counter to the next: a cache line each, so that rows do not wait for one another
-constexpr int slice_of(int threads) { return threads * 4 * AHEAD; }
+constexpr int MOST_SLICE = THREADS * 4 * AHEAD, LEAST_SLICE = THREADS * 4;
 // four numbers wherever they begin
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -118,8 +116,8 @@ __device__ __forceinline__ int best_of_row(const unsigned long long* best, int n
 // Grid (slices of a row, rows), a workgroup each.  CHOOSE: its best candidate to best [rows, workgroups], or,
 // of a row that has one workgroup, the token to ``chosen``; else the adjusted logits to ``out``.  With ``arrived`` (a counter a
 // row, 0 before and after) the last workgroup of a row to arrive joins the row's candidates: one launch instead of two.
-template <bool CHOOSE, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == PART_THREADS ? (CHOOSE ? 8 : 5) : 4)
+template <bool CHOOSE>
+__global__ void __launch_bounds__(THREADS, 8)
 rules_kernel(const float* logits, long ld, Rules rules, int V, int slice, float* out, long out_ld,
              const float* __restrict__ temperatures, const long long* __restrict__ seeds, const int* __restrict__ counters,
              unsigned long long* best, int* arrived, int* __restrict__ chosen) {
@@ -316,14 +314,12 @@ record_tokens_kernel(int* __restrict__ history, long ld, int slots, int most, co
 
 MIE_EXPORT const char* logit_rules_last_error() { return g_mie_error; }
 
-// Tokens a workgroup takes.  The whole of a short row, which one workgroup goes through in less time than several take to meet (choosing, alone, 1 to
-// 256 rows of 5,000: one workgroup 12.9 to 15.1 us, two slices 14.8 to 19.3).  Else slices, shorter ones as long as they are few: choosing from 1 row
-// of 32,000 18.1 us with slices of 4,096, 13.8 of 1,024, 32 rows 16.7 and 13.7, 64 rows 19.0 and (2,048) 16.6; four a compute unit are
-// enough, at eight every text is read too often (32 rows of 128,256 20.5 us, 23.8).
+// Tokens a workgroup takes: fewer as long as the workgroups are few.  (Kernels alone, us, choosing and adjusting: 8 rows of 8,000 6.5 and 4.2, 9.8 and 6.1
+// a row in one workgroup of 1,024 threads, 256 rows of 5,000 9.1 and 6.6 where those take 8.4 and 6.1.)  Four a compute unit are enough, at eight every text is read too
+// often (32 rows of 128,256 12.0, 15.8), at two the units are not filled (64 rows of 32,000 9.5, 10.9).
 static int slice_for(int rows, int V) {
-  if (V <= 2 * slice_of(PART_THREADS)) return (V + 3) & ~3;
-  int slice = slice_of(PART_THREADS);
-  while (slice > PART_THREADS * 4 && (long)rows * ((V + slice - 1) / slice) < 4L * mie_compute_units()) slice /= 2;
+  int slice = MOST_SLICE;
+  while (slice > LEAST_SLICE && (long)rows * ((V + slice - 1) / slice) < 4L * mie_compute_units()) slice /= 2;
   return slice;
 }
 
@@ -348,11 +344,7 @@ static int launch_rules(const char* what, const float* logits, long ld, const Ru
   if (rows <= 0) return 0;
   if (check_rules(what, rules, rows, V, ld)) return -1;
   const int slice = slice_for(rows, V), slices = (V + slice - 1) / slice;
-  const int threads = slices > 1 ? PART_THREADS : ROW_THREADS;
-  const int lds = slice * 4;
-  auto* kernel = slices > 1 ? rules_kernel<CHOOSE, PART_THREADS> : rules_kernel<CHOOSE, ROW_THREADS>;
-  if (lds > 65536 - 256 && mie_allow_lds(reinterpret_cast<const void*>(kernel), lds, what)) return -1;
-  hipLaunchKernelGGL(kernel, dim3(slices, rows), dim3(threads), lds, stream, logits, ld, rules, V, slice, out, out_ld, temperatures,
+  hipLaunchKernelGGL(rules_kernel<CHOOSE>, dim3(slices, rows), dim3(THREADS), slice * 4, stream, logits, ld, rules, V, slice, out, out_ld, temperatures,
                      seeds, counters, best, arrived, chosen);
   MIE_CHECK_LAUNCH(what);
   if (CHOOSE && slices > 1 && !arrived) {
