@@ -24,7 +24,7 @@
 // of own keys alone take 110 (about the rate of a large copy), the 34 GFLOP over shared keys alone 67, hidden behind them as long as the own keys'
 // waves, which wait for no other wave, share the units (with four waves a row 131 to 141).  Many columns alone are a chain of LDS reads, products and
 // softmax: of 1,024 keys of 128 a workgroup of 128 columns takes 34 us by itself, two on a unit 51.  8 rows behind 30,000 keys 32.5 us for 134 MB (4.1
-// TB/s).  32 rows behind 2,000 keys 20 us, 4 of them the join: a workgroup's first loads, last stores and one stage take 7 us.
+// TB/s).  32 rows behind 2,000 keys 18 to 19 us, 4 of them the join: a workgroup's first loads, last stores and one stage take 7 us.
 #include "attention_bf16_common.hpp"
 #include "launch.hpp"
 #include <type_traits>

@@ -18,7 +18,7 @@ BLOCK_KEYS = 32
 LEAST_KEYS = 64         # of a cut: an item's start and its partial result cost about as much
 START = 500             # what a workgroup's start and end cost, in keys of an item of up to 16 columns
 LEAST_WIDE_KEYS = 192   # the same of items of more than 64 columns in bfloat16, whose partial results are the larger (32 rows behind 2,000
-                        # keys: cuts of 64 keys 22 us, of 128 18.7, of 192 17.1, of 256 18.8)
+                        # keys in such items: cuts of 64 keys 22 us, of 128 18.7, of 192 17.1, of 256 18.8)
 
 
 def _sharers(head_dim: int, float32: bool) -> int:
@@ -64,15 +64,22 @@ class SharedPrefixPlan:
                 work.append((first, n * G, 0, k))
             work += [(r, G, k, contexts[r]) for r in range(first, first + n) if contexts[r] > k]
             first += n
-        widest = max((w[1] for w in work), default=1)
-        self.column_tiles = 2 if widest > TILE and head_dim <= 128 and not float32 else 1
-        wide = TILE * self.column_tiles
-        tiles = [-(-w[1] // wide) for w in work]
         # What a key of an item costs, in keys of an item of up to 16 columns, whose waves share out the keys: measured, us for 64 keys in
         # bfloat16 0.4, of up to 64 columns 0.9, of 128 columns 1.3 (head size 128); the products of float32 weigh more.
-        wider = 4 if float32 else 2
-        cost = [1 if w[1] <= 16 else wider if min(w[1], wide) <= TILE else 3 for w in work]
-        total = sum(t * c * (w[3] - w[2]) for w, t, c in zip(work, tiles, cost)) * num_kv_heads
+        def weigh(column_tiles):
+            wide = TILE * column_tiles
+            tiles = [-(-w[1] // wide) for w in work]
+            cost = [1 if w[1] <= 16 else (4 if float32 else 2) if min(w[1], wide) <= TILE else 3 for w in work]
+            return wide, tiles, cost, sum(t * c * (w[3] - w[2]) for w, t, c in zip(work, tiles, cost)) * num_kv_heads
+
+        # 128 columns a workgroup cost less than twice 64, but where there is little to do 64 leave the keys in fewer pieces to join (32 rows of 32 / 8
+        # heads behind 2,000 keys, 190 keys a unit by these weights, 17.8 us and 19.2; 172 of 8 / 2 behind some 3,200, 450, 20.3 and 22.7; 2 times 107
+        # of 32 / 4 behind some 800, 530, 19.7 and 18.2; 126 of 8 / 2 behind 16,712, 1,570, 26.9 and 23.5).
+        self.column_tiles = 2 if max((w[1] for w in work), default=1) > TILE and head_dim <= 128 and not float32 else 1
+        wide, tiles, cost, total = weigh(self.column_tiles)
+        if self.column_tiles == 2 and total <= 600 * units:
+            self.column_tiles = 1
+            wide, tiles, cost, total = weigh(1)
         # One compute unit's share.  Items of half of it balance better and leave twice the partial results: over fifteen shapes in
         # geometric mean 35.3 us, 33.2 at two thirds, 31.9 at this, 33.9 at four thirds.  But two workgroups on a unit do 1.35 times what one does, which
         # long items are worth cutting for (two thirds: 256 rows behind 8,192 keys 118 -> 109 us, 77 of 56 / 7 heads of 32 behind 20,855 63 -> 53).
