@@ -17,7 +17,7 @@ import pytest
 import torch
 
 from mini_inference_engine_amd.kernels.hip_backend import HipBackend
-from mini_inference_engine_amd.kernels.shared_prefix import SharedPrefixPlan
+from mini_inference_engine_amd.kernels.shared_prefix import SharedPrefixPlan, _sharers
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -144,6 +144,45 @@ def test_shared_prefix_attention(ops, case, heads, dtype):
     groups, own = GROUPS[case]
     s = make(groups, rows_behind(groups, own, case), *heads, 16, dtype, seed=case)
     run(ops, s, groups, *heads, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads", [(2, 1, 16), (3, 3, 32), (4, 2, 48), (32, 4, 64), (6, 2, 96), (8, 2, 128), (16, 1, 128), (20, 1, 64), (2, 2, 256), (8, 1, 256)])
+@pytest.mark.parametrize("case", range(len(GROUPS)))
+def test_items_of_a_wave_and_of_more_columns(ops, case, heads, dtype):
+    """Plans for a few compute units: short rows a wave each, and, for some hundred, items as short as they get."""
+    groups, own = GROUPS[case]
+    Hq, Hkv, D = heads
+    s = make(groups, rows_behind(groups, own, case), *heads, 16, dtype, seed=case)
+    contexts = [p + 1 for p in s.positions.tolist()]
+    waves = _sharers(D, dtype == F32) if Hq // Hkv <= 16 else 0
+    for nobody in (False, True):
+        if nobody:                              # padding in between, and a row in the middle of its own keys
+            s.positions[::3] = -1
+            s.positions[-1] = max(0, int(s.positions[-1]) - 5) if int(s.positions[-1]) - 5 >= groups[-1][1] else int(s.positions[-1])
+        step, group = step_of(s, most=max(contexts))
+        want = plain(s, *heads, D ** -0.5, 0.3)
+        for units in (1, 7, 600):
+            for share in (True, False):
+                plan = SharedPrefixPlan(groups, contexts, *heads, "cuda", units=units, float32=dtype == F32, share=share)
+                if units == 1:
+                    alone = sum(c <= Hq // Hkv for _, c, *_ in plan.items.view(-1, 8).tolist())
+                    assert plan.num_items - plan.whole_items <= alone and (waves > 0 or plan.whole_items == plan.num_items)
+                check(ops[dtype].shared_prefix_attention(s.q, *heads, s.k, s.v, group, step, D ** -0.5, plan, sink=0.3), *want, D, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads", [(8, 8, 64), (16, 4, 128), (4, 4, 256)])
+def test_hundreds_of_short_rows(ops, heads, dtype):
+    """More workgroups than there is room for: rows of 1 to 460 keys, whole and behind some shared ones, a wave each."""
+    g = np.random.RandomState(1)
+    for groups in ([(300, 0)], [(130, 48), (1, 0), (200, 16)]):
+        positions = [k + int(x) - 1 for n, k in groups for x in g.choice([1, 2, 31, 32, 33, 100, 440], n)]
+        s = make(groups, positions, *heads, 16, dtype, poison=False)
+        out, plan = run(ops, s, groups, *heads, dtype)
+        assert plan.num_items - plan.whole_items > 100
 
 
 @pytest.mark.gpu
@@ -434,6 +473,8 @@ def covered(plan, groups, contexts, G):
                 assert at == contexts[r]
         first += n
     assert plan.num_parts == starts[-1] and plan.join == any(b - a != 1 for a, b in zip(starts, starts[1:]))
+    waves = items[plan.whole_items:]         # one row each, the longest first
+    assert all(columns == G <= 16 for _, columns, *_ in waves) and [e - b for _, _, _, b, e, *_ in waves] == sorted((e - b for _, _, _, b, e, *_ in waves), reverse=True)
     first = 0
     for n, keys in groups:                   # an item of several rows holds shared keys only
         for row, columns, _, begin, end, _, _, _ in items:
@@ -449,7 +490,7 @@ def test_a_plan_covers_every_key_once(seed, share):
     groups = [(int(g.randint(1, 40)), int(g.choice([0, 1, 31, 32, 500, 7000, 40000]))) for _ in range(g.randint(1, 6))]
     contexts = [k + int(g.choice([0, 1, 2, 33, 900])) for n, k in groups for _ in range(n)]
     G, Hkv = int(g.choice([1, 3, 8, 16])), int(g.choice([1, 4, 8]))
-    plan = SharedPrefixPlan(groups, contexts, G * Hkv, Hkv, 64, "cpu", float32=bool(seed % 2), share=share)
+    plan = SharedPrefixPlan(groups, contexts, G * Hkv, Hkv, 64, "cpu", units=256 if seed < 30 else 4, float32=bool(seed % 2), share=share)
     covered(plan, groups, contexts, G)
     shared = any(columns > G for _, columns, *_ in plan.items.view(-1, 8).tolist())
     if share is not None:
