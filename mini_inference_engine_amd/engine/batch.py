@@ -64,15 +64,26 @@ class StepContext:
     host: dict = field(default_factory=dict)   # the same arrays as numpy, for parts that plan on the host
     shared_prefix: list | None = None   # (rows, keys) of runs of rows that share their first keys (ModelRunner.forward_step)
     prefix_plans: dict = field(default_factory=dict)   # of that, by heads
+    kept_plans: dict = field(default_factory=dict)     # the same of earlier steps, with what they were made for (the runner's)
     shared: dict = field(default_factory=dict)  # what one layer of the step leaves for later ones, by name (tensors over the
                                                 # step's tokens; a layer that gives writes it anew in every forward)
 
     def prefix_plan(self, ops, num_q_heads: int, num_kv_heads: int, head_dim: int):
-        """The backend's plan of ``shared_prefix`` for layers with such heads, made by the first of them."""
+        """The backend's plan of ``shared_prefix`` for layers with such heads, made by the first of them: for contexts that are a
+        little longer, so that the steps that follow with the same runs of rows find it made (256 rows: 0.5 ms on the host)."""
         key = (num_q_heads, num_kv_heads, head_dim)
-        if key not in self.prefix_plans:
-            self.prefix_plans[key] = ops.plan_shared_prefix(self.shared_prefix, self.host["row_context"], *key)
-        return self.prefix_plans[key]
+        plan = self.prefix_plans.get(key)
+        if plan is None:
+            ends = self.host["row_context"]
+            runs, contexts, plan = self.kept_plans.get(key, (None, None, None))
+            if runs != self.shared_prefix or (contexts < ends).any() or (contexts - ends > 2 * self.PLANNED_AHEAD).any():
+                contexts = np.minimum(ends + self.PLANNED_AHEAD, max(g.max_blocks for g in self.groups) * self.page_size)
+                plan = ops.plan_shared_prefix(self.shared_prefix, contexts, *key)
+                self.kept_plans[key] = list(self.shared_prefix), contexts, plan
+            self.prefix_plans[key] = plan
+        return plan
+
+    PLANNED_AHEAD = 64
 
 
 class StepArena:

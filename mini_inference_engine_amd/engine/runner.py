@@ -106,6 +106,7 @@ class ModelRunner:
         # The tokens the last step chose, at a fixed address: the next step's rows may take their token
         # from here on the device (StepRow.taken_from) before the host has seen it.
         self.chosen_tokens = torch.zeros(max(1, max_rows), dtype=torch.int32, device=self.device)
+        self.prefix_plans = {}              # of steps with shared first parts, by heads (StepContext.prefix_plan)
         self.token_history = None           # [slots, positions] int32: every request's tokens (keep_token_history)
         self.graphs = None                  # captured decode steps, once capture_decode_graphs was called
         self.portion_graphs = []            # captured steps of one prompt portion, by token count (capture_portion_graphs)
@@ -211,7 +212,8 @@ class ModelRunner:
                 return logits
         else:
             step = self.build(rows, sampling=sampling)
-            step.shared_prefix = shared_prefix
+            if shared_prefix is not None:
+                step.shared_prefix, step.kept_plans = list(shared_prefix), self.prefix_plans
             with self.ranges("forward"):
                 logits = self.model.forward(step)
         if sampling is not None and logits is not None:

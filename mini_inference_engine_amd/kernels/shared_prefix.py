@@ -36,22 +36,22 @@ class SharedPrefixPlan:
 
     def __init__(self, groups, contexts, num_q_heads: int, num_kv_heads: int, head_dim: int, device, units: int = 256,
                  float32: bool = False, share: bool | None = None):
-        contexts = [int(c) for c in contexts]
+        self.contexts = np.array(contexts, dtype=np.int64).reshape(-1)
+        contexts = self.contexts.tolist()
         groups = [(int(n), int(k)) for n, k in groups]
         if num_kv_heads < 1 or num_q_heads < 1 or num_q_heads % num_kv_heads:
             raise ValueError(f"shared prefix: {num_q_heads} query heads are not a multiple of {num_kv_heads} kv heads")
         if any(n < 1 or k < 0 for n, k in groups) or sum(n for n, _ in groups) != len(contexts):
             raise ValueError(f"shared prefix: runs of rows {groups[:8]} for {len(contexts)} rows")
-        if any(c < 0 or c > 0x7FFFFF00 for c in contexts):
+        self.max_context = max(contexts, default=0)
+        if min(contexts, default=0) < 0 or self.max_context > 0x7FFFFF00:
             raise ValueError("shared prefix: contexts are numbers of keys, 0 or more")
         first = 0
         for n, k in groups:
-            if any(c < k for c in contexts[first:first + n]):
+            if min(contexts[first:first + n]) < k:
                 raise ValueError(f"shared prefix: rows {first} to {first + n - 1} share {k} keys, and one of them has fewer")
             first += n
         self.num_rows, self.num_q_heads, self.num_kv_heads, self.head_dim = len(contexts), int(num_q_heads), int(num_kv_heads), int(head_dim)
-        self.contexts = np.asarray(contexts, dtype=np.int64)
-        self.max_context = max(contexts, default=0)
         G = num_q_heads // num_kv_heads
         whole = not self._worth_it(G, units, float32) if share is None else not share
         if whole:
@@ -87,7 +87,7 @@ class SharedPrefixPlan:
         if most > 3000:
             most = -(-2 * most // 3)
 
-        parts = np.zeros(self.num_rows, dtype=np.int64)
+        parts = [0] * self.num_rows
         items, several, solo = [], [], []
         # Rows whose own keys are few next to a compute unit's share get a wave each: fewer workgroups, and nothing to join among the waves.  (236
         # rows of 48 / 6 heads of 64 behind 2,466 keys with 1 to 75 of their own 40.4 -> 37.8 us, 248 rows of 21 / 7 of 256 behind some 770 with
@@ -102,18 +102,18 @@ class SharedPrefixPlan:
             least = LEAST_WIDE_KEYS if c == 3 else LEAST_KEYS
             pieces = 1 if whole and share is None else -(-(end - begin) // max(least, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
             size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
-            rows = columns // G
-            at = begin
+            rows, at, part = columns // G, begin, parts[row]
             if rows == 1 and pieces == 1 and end - begin <= few:
-                solo.append((row, columns, 0, begin, end, int(parts[row]), 0, 0))
-                parts[row] += 1
+                solo.append((row, columns, 0, begin, end, part, 0, 0))
+                parts[row] = part + 1
                 continue
             while at < end:
                 # cuts lie on whole blocks of the cache, so that no block is read twice
                 to = end if end - at <= size else (at + size) // BLOCK_KEYS * BLOCK_KEYS
-                (several if rows > 1 else items).extend((row, columns, i * wide, at, to, int(parts[row]), 0, 0) for i in range(t))
-                parts[row:row + rows] += 1
+                (several if rows > 1 else items).extend([(row, columns, i * wide, at, to, part, 0, 0) for i in range(t)])
+                part += 1
                 at = to
+            parts[row:row + rows] = [part] * rows
         # the longest first: items of many columns take several times what those of one row do (256 rows behind 8,192 keys: the two kinds
         # spread among one another 256 us, these first 182)
         items = several + items
@@ -123,7 +123,8 @@ class SharedPrefixPlan:
         starts = np.zeros(self.num_rows + 1, dtype=np.int32)
         np.cumsum(parts, out=starts[1:])
         self.num_parts = int(starts[-1])
-        self.most_parts = 1 if (parts == 1).all() else max(2, int(parts.max()))      # 1: every row has one, nothing to join
+        most_parts = max(parts, default=1)
+        self.most_parts = 1 if most_parts == min(parts, default=1) == 1 else max(2, most_parts)      # 1: every row has one, nothing to join
         self.join = self.most_parts != 1
         packed = np.concatenate([np.asarray(items, dtype=np.int32).reshape(-1), starts])
         data = torch.from_numpy(packed)

@@ -15,7 +15,7 @@ from torch_backend import TorchBackend, ref_perturbed
 
 from mini_inference_engine_amd import SamplingParams
 from mini_inference_engine_amd.cache import CacheAccountingError, CacheManager, GroupSpec
-from mini_inference_engine_amd.engine.batch import StepRow
+from mini_inference_engine_amd.engine.batch import StepContext, StepRow
 from mini_inference_engine_amd.engine.runner import ModelRunner
 from mini_inference_engine_amd.sampling import RuleInputs
 
@@ -204,7 +204,40 @@ def answers_to(m, device, dtype, slack, weights, prompt_tokens, steps=10, alone=
 @pytest.mark.parametrize("prompt_tokens", [49, 70, 12])
 def test_answers_host(tiny_models, model, prompt_tokens):
     runner = answers_to(tiny_models[model], "cpu", "float32", 1e-5, "weights", prompt_tokens)
-    assert runner.ops.calls["shared"] > 0 and runner.ops.calls["plan"] == 10      # one plan a step, for all its layers
+    assert runner.ops.calls["shared"] > 0 and runner.ops.calls["plan"] == 1       # one plan for all layers of ten steps
+
+
+def test_a_plan_is_kept_as_long_as_it_fits(tiny_models, monkeypatch):
+    m = tiny_models["A"]
+    monkeypatch.setattr(StepContext, "PLANNED_AHEAD", 16)
+    runner = ModelRunner(m["config"], backend=SharedBackend(torch.float32), weights=m["weights"], dtype="float32", device="cpu", num_pages=60,
+                         page_size=16, max_step_tokens=256, max_rows=4)
+    a, b, c = (runner.cache.open(x) for x in "abc")
+    prompt = prompts_for(m, [40])[0]
+    for rc in (a, c):
+        assert runner.cache.reserve(rc, 0, runner.max_model_len)
+        runner.forward_step([StepRow(rc, prompt, 0)])
+    runner.cache.close(b)
+    b = runner.cache.fork(a, "d", 40)
+    assert runner.cache.reserve(b, 32, 100)
+    runner.forward_step([StepRow(b, prompt[32:], 32)])
+
+    def plans(starts, runs, first=a):
+        before = runner.ops.calls.get("plan", 0)
+        rows = [StepRow(rc, [1], s, [0]) for rc, s in zip((first, b, c), starts)]
+        logits = runner.forward_step(rows, shared_prefix=runs)
+        assert torch.allclose(logits, runner.forward_step(rows), atol=1e-5 * float(logits.abs().max()))
+        return runner.ops.calls.get("plan", 0) - before
+
+    runs, last = [(2, 32), (1, 0)], runner.max_model_len - 1
+    assert plans((40, 40, 40), runs) == 1
+    assert plans((41, 41, 41), tuple(runs)) == 0 and plans((56, 41, 56), runs) == 0
+    assert plans((57, 41, 40), runs) == 1                       # a row beyond what was planned
+    assert plans((57, 41, 40), [(2, 16), (1, 0)]) == 1          # other runs
+    assert plans((57, 41, 40), runs) == 1
+    assert plans((40, 40, 40), runs) == 1                       # a row far short of what was planned
+    assert plans((40, 40), [(2, 32)]) == 1
+    assert plans((last, 100, last), runs) == 1                  # planned no further than the block tables go
 
 
 def test_refused_shared_steps(tiny_models):
