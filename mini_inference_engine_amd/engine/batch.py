@@ -38,6 +38,20 @@ class GroupStep:
 
 
 @dataclass
+class KeptPlan:
+    """A plan of shared first parts with what it was made for."""
+    AHEAD = 64                       # keys that contexts are planned longer than they are
+
+    runs: list
+    contexts: np.ndarray
+    plan: object
+
+    def fits(self, runs, ends) -> bool:
+        """Whether steps with such runs of rows and contexts can go on with it: none beyond what was planned, none far short of it."""
+        return self.runs == runs and bool((self.contexts >= ends).all() and (self.contexts - ends <= 2 * self.AHEAD).all())
+
+
+@dataclass
 class StepContext:
     num_tokens: int
     num_rows: int
@@ -74,16 +88,12 @@ class StepContext:
         key = (num_q_heads, num_kv_heads, head_dim)
         plan = self.prefix_plans.get(key)
         if plan is None:
-            ends = self.host["row_context"]
-            runs, contexts, plan = self.kept_plans.get(key, (None, None, None))
-            if runs != self.shared_prefix or (contexts < ends).any() or (contexts - ends > 2 * self.PLANNED_AHEAD).any():
-                contexts = np.minimum(ends + self.PLANNED_AHEAD, max(g.max_blocks for g in self.groups) * self.page_size)
-                plan = ops.plan_shared_prefix(self.shared_prefix, contexts, *key)
-                self.kept_plans[key] = list(self.shared_prefix), contexts, plan
-            self.prefix_plans[key] = plan
+            ends, kept = self.host["row_context"], self.kept_plans.get(key)
+            if kept is None or not kept.fits(self.shared_prefix, ends):
+                contexts = np.minimum(ends + KeptPlan.AHEAD, max(g.max_blocks for g in self.groups) * self.page_size)
+                kept = self.kept_plans[key] = KeptPlan(list(self.shared_prefix), contexts, ops.plan_shared_prefix(self.shared_prefix, contexts, *key))
+            plan = self.prefix_plans[key] = kept.plan
         return plan
-
-    PLANNED_AHEAD = 64
 
 
 class StepArena:

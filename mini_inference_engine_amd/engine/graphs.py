@@ -93,6 +93,48 @@ class DecodeGraphs:
         return logits[torch.tensor(picked, device=logits.device)], step
 
 
+class SharedGraph:
+    """The captured step of single-token rows that share first parts of their caches, under plans made for an earlier step
+    (StepContext.prefix_plan): it serves steps as long as those plans do.  Captured when the second such step comes, that is once for some
+    sixty steps of one set of rows (22 layers at TinyLlama sizes: 10 ms)."""
+
+    def __init__(self, runner, rows, runs):
+        self.plans = [k.plan for k in runner.prefix_plans.values()]      # (held: the graph reads their memory)
+        self.rows = len(rows)
+        self.static_context = min(int(k.contexts.max()) for k in runner.prefix_plans.values())
+        step = self._build(runner, rows, None)
+        step.shared_prefix, step.kept_plans = runs, runner.prefix_plans
+        torch.cuda.synchronize()
+        self.graph = torch.cuda.CUDAGraph()
+        collecting = gc.isenabled()
+        gc.disable()                                    # (as for the decode graphs: nothing is collected while the stream records)
+        try:
+            with torch.cuda.graph(self.graph):
+                self.logits = runner.model.forward(step)
+        finally:
+            if collecting:
+                gc.enable()
+        torch.cuda.synchronize()
+
+    def _build(self, runner, rows, sampling):
+        return runner.build(rows, pad_rows_to=len(rows), static_context=self.static_context, want_all=True, sampling=sampling)
+
+    def fits(self, runner, rows) -> bool:
+        return self.rows == len(rows) and len(self.plans) == len(runner.prefix_plans) and all(a is b.plan for a, b in zip(self.plans, runner.prefix_plans.values()))
+
+    def run(self, runner, rows, sampling=None):
+        """As DecodeGraphs.run; tokens are chosen behind the graph."""
+        picked = [i for i, r in enumerate(rows) if len(r.want)]
+        step = self._build(runner, rows, sampling)
+        with runner.ranges("forward"):
+            self.graph.replay()
+        if not picked:
+            return None, step
+        if len(picked) == len(rows):
+            return self.logits, step
+        return self.logits[torch.tensor(picked, device=self.logits.device)], step
+
+
 class _ScratchRequest:
     """What a row needs of a request's cache, all of it the scratch page and the scratch slot: the row a step is
     captured with."""

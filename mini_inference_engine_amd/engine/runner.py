@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import contextlib
 
+import numpy as np
 import torch
 
 from ..cache import CacheManager, CacheStorage, GroupSpec
@@ -107,6 +108,7 @@ class ModelRunner:
         # from here on the device (StepRow.taken_from) before the host has seen it.
         self.chosen_tokens = torch.zeros(max(1, max_rows), dtype=torch.int32, device=self.device)
         self.prefix_plans = {}              # of steps with shared first parts, by heads (StepContext.prefix_plan)
+        self.shared_graph = None            # the captured step that goes on with them
         self.token_history = None           # [slots, positions] int32: every request's tokens (keep_token_history)
         self.graphs = None                  # captured decode steps, once capture_decode_graphs was called
         self.portion_graphs = []            # captured steps of one prompt portion, by token count (capture_portion_graphs)
@@ -195,14 +197,24 @@ class ModelRunner:
 
         ``shared_prefix``: (rows, keys) of runs of rows, in order, that hold the same pages for their first ``keys``
         tokens (CacheManager.fork; whole pages, 0: nothing shared), for a step of single-token rows: layers that see all
-        earlier keys then read the shared ones once a run (KernelBackend.shared_prefix_attention).  Such a step is not a captured one."""
+        earlier keys then read the shared ones once a run (KernelBackend.shared_prefix_attention).  Where decode steps are captured, the
+        second step of the same runs is as well, and serves those after it."""
         if shared_prefix is not None:
+            shared_prefix = list(shared_prefix)
             self._check_shared_prefix(rows, shared_prefix)
         self.last_step_captured = False
         captured = (shared_prefix is None and self.graphs is not None and self.graphs.fits(len(rows)) and all(len(r.tokens) == 1 for r in rows)
                     and (sampling is None or all(len(r.want) == 1 for r in rows)))
         portion = None if captured or shared_prefix is not None or not self.portion_graphs else self._portion_graph_for(rows)
-        if portion is not None:
+        if shared_prefix is not None and self._plans_go_on(rows, shared_prefix, sampling):
+            if self.shared_graph is None or not self.shared_graph.fits(self, rows):
+                from .graphs import SharedGraph
+                torch.cuda.synchronize()
+                self.shared_graph = None                                 # (no longer running: what it holds is free for the next)
+                self.shared_graph = SharedGraph(self, rows, shared_prefix)
+            self.last_step_captured = True
+            logits, step = self.shared_graph.run(self, rows, sampling)
+        elif portion is not None:
             self.last_step_captured = True
             logits, step = portion.run(self, rows, sampling)
         elif captured:
@@ -213,7 +225,7 @@ class ModelRunner:
         else:
             step = self.build(rows, sampling=sampling)
             if shared_prefix is not None:
-                step.shared_prefix, step.kept_plans = list(shared_prefix), self.prefix_plans
+                step.shared_prefix, step.kept_plans = shared_prefix, self.prefix_plans
             with self.ranges("forward"):
                 logits = self.model.forward(step)
         if sampling is not None and logits is not None:
@@ -223,6 +235,15 @@ class ModelRunner:
                 self.ops.sample(logits, step.sample_temps[:n], step.sample_seeds[:n], step.sample_counters[:n],
                                 out=self.chosen_tokens[:n], **under)
         return logits
+
+    def _plans_go_on(self, rows, runs, sampling) -> bool:
+        """Whether a step with shared first parts can be captured, or is: the plans of an earlier one fit it."""
+        if self.graphs is None or not self.graphs.sizes or not self.prefix_plans:
+            return False
+        if any(len(r.want) > 1 or (sampling is not None and not len(r.want)) for r in rows):
+            return False
+        ends = np.array([r.start + 1 for r in rows])
+        return all(kept.fits(runs, ends) for kept in self.prefix_plans.values())
 
     def _check_shared_prefix(self, rows, runs) -> None:
         if any(len(r.tokens) != 1 for r in rows) or sum(n for n, _ in runs) != len(rows) or any(n < 1 for n, _ in runs):

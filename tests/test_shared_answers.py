@@ -15,7 +15,7 @@ from torch_backend import TorchBackend, ref_perturbed
 
 from mini_inference_engine_amd import SamplingParams
 from mini_inference_engine_amd.cache import CacheAccountingError, CacheManager, GroupSpec
-from mini_inference_engine_amd.engine.batch import StepContext, StepRow
+from mini_inference_engine_amd.engine.batch import KeptPlan, StepRow
 from mini_inference_engine_amd.engine.runner import ModelRunner
 from mini_inference_engine_amd.sampling import RuleInputs
 
@@ -178,7 +178,7 @@ def answers_to(m, device, dtype, slack, weights, prompt_tokens, steps=10, alone=
         sampling = ([a.params.temperature for a in answers], [a.params.seed or 0 for a in answers], [a.num_output_tokens for a in answers])
         rules = inputs.make(answers, [len(a.tokens) for a in answers], history)
         logits = runner.forward_step(rows, sampling=sampling, rules=rules, shared_prefix=runs)
-        assert not runner.last_step_captured
+        assert runner.last_step_captured == (graphs and step > 0)
         chosen = runner.chosen_tokens[:len(answers)].tolist()
         if step == 0:                # the same step without sharing (its keys and values are written over with the same ones)
             again = runner.forward_step(rows, sampling=sampling, rules=rules)
@@ -209,7 +209,7 @@ def test_answers_host(tiny_models, model, prompt_tokens):
 
 def test_a_plan_is_kept_as_long_as_it_fits(tiny_models, monkeypatch):
     m = tiny_models["A"]
-    monkeypatch.setattr(StepContext, "PLANNED_AHEAD", 16)
+    monkeypatch.setattr(KeptPlan, "AHEAD", 16)
     runner = ModelRunner(m["config"], backend=SharedBackend(torch.float32), weights=m["weights"], dtype="float32", device="cpu", num_pages=60,
                          page_size=16, max_step_tokens=256, max_rows=4)
     a, b, c = (runner.cache.open(x) for x in "abc")
@@ -270,3 +270,56 @@ def test_refused_shared_steps(tiny_models):
 @pytest.mark.parametrize("dtype, slack, weights", [("float32", 1e-5, "weights"), ("bfloat16", 2e-2, "weights_bf16")])
 def test_answers_gpu(tiny_models, model, dtype, slack, weights, graphs, share):
     answers_to(tiny_models[model], "cuda", dtype, slack, weights, 70, graphs=graphs, share=share)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("model", ["A", "B", "C"])
+@pytest.mark.parametrize("dtype, slack, weights", [("float32", 1e-5, "weights"), ("bfloat16", 2e-2, "weights_bf16")])
+def test_captured_steps_of_shared_first_parts(tiny_models, monkeypatch, model, dtype, slack, weights):
+    """Steps replayed under kept plans are what they are kernel by kernel, over new plans, other rows, rows without wishes and back."""
+    m = tiny_models[model]
+    monkeypatch.setattr(KeptPlan, "AHEAD", 5)
+    runner = ModelRunner(m["folder_f32"] if dtype == "float32" else m["folder_bf16"], dtype=dtype, num_pages=60, page_size=16, max_step_tokens=256,
+                         max_rows=8)
+    runner.capture_decode_graphs((2, 8), sample=True)
+    runner.ops.plan_shared_prefix = functools.partial(runner.ops.plan_shared_prefix, share=True)
+    prompt = prompts_for(m, [49], seed=3)[0]
+    first = runner.cache.open("p")
+    assert runner.cache.reserve(first, 0, 49)
+    runner.forward_step([StepRow(first, prompt[:48], 0)])
+    caches = [runner.fork(first, i, 48) for i in range(4)]
+    for rc in caches:
+        assert runner.cache.reserve(rc, 48, 40)
+
+    def step(k, who, runs, want=None, sample=True):
+        rows = [StepRow(caches[i], [7 + 3 * i + k], 48 + k, [] if want is not None and i not in want else [0]) for i in who]
+        n = sum(len(r.want) for r in rows)
+        sampling = ([0.7] * n, list(range(n)), [k] * n) if sample else None
+        got = runner.forward_step(rows, sampling=sampling, shared_prefix=runs)
+        captured, chosen = runner.last_step_captured, runner.chosen_tokens[:n].tolist()
+        if got is not None:
+            got = got.clone()
+        graphs, runner.graphs = runner.graphs, None
+        want_logits = runner.forward_step(rows, sampling=sampling, shared_prefix=runs)
+        runner.graphs = graphs
+        if got is None:
+            assert want_logits is None
+        else:
+            # (the step kernel by kernel may split a matrix product otherwise than a captured one)
+            assert got.shape == want_logits.shape and float((got - want_logits).abs().max()) <= slack * float(want_logits.abs().max())
+            if sample and torch.equal(got, want_logits):
+                assert chosen == runner.chosen_tokens[:n].tolist()
+        return captured
+
+    runs = [(3, 48), (1, 0)]
+    assert [step(k, range(4), runs) for k in range(5)] == [False, True, True, True, True]
+    graph = runner.shared_graph
+    assert step(5, range(4), runs) and runner.shared_graph is graph
+    assert not step(6, range(4), runs) and step(7, range(4), runs) and runner.shared_graph is not graph       # beyond what was planned
+    assert not step(8, (0, 2), [(2, 48)]) and step(8, (0, 2), [(2, 48)])
+    assert step(9, (0, 2), [(2, 48)], want=(2,), sample=False) and step(9, (0, 2), [(2, 48)], want=(), sample=False)
+    assert not step(9, (0, 2), [(2, 48)], want=(2,))                   # choices for some rows only: kernel by kernel
+    assert not step(10, range(4), runs) and step(11, range(4), tuple(runs))
+    for rc in [first, *caches]:
+        runner.cache.close(rc)
+    runner.cache.check()
