@@ -200,7 +200,7 @@ class ModelRunner:
         earlier keys then read the shared ones once a run (KernelBackend.shared_prefix_attention).  Where decode steps are captured, the
         second step of the same runs is as well, and serves those after it."""
         if shared_prefix is not None:
-            shared_prefix = list(shared_prefix)
+            shared_prefix = [(int(n), int(keys)) for n, keys in shared_prefix]
             self._check_shared_prefix(rows, shared_prefix)
         self.last_step_captured = False
         captured = (shared_prefix is None and self.graphs is not None and self.graphs.fits(len(rows)) and all(len(r.tokens) == 1 for r in rows)
