@@ -87,8 +87,6 @@ class SharedPrefixPlan:
         if most > 3000:
             most = -(-2 * most // 3)
 
-        parts = [0] * self.num_rows
-        items, several, solo = [], [], []
         # Rows whose own keys are few next to a compute unit's share get a wave each: fewer workgroups, and nothing to join among the waves.  (236
         # rows of 48 / 6 heads of 64 behind 2,466 keys with 1 to 75 of their own 40.4 -> 37.8 us, 248 rows of 21 / 7 of 256 behind some 770 with
         # 1 to 63 79 -> 53; the 256 rows below 131 -> 116; 220 rows of 15 / 5 of 128 with 200 to 220 keys, whole, 20 -> 15, with 800 39 -> 43.)  Of
@@ -98,22 +96,33 @@ class SharedPrefixPlan:
         few = (share_with_starts - START) / (2 * sharers) if sharers else 0
         if sharers and sum(w[1] == G for w in work) * num_kv_heads > 2 * units:
             few = max(few, 224 if float32 and sharers < 4 else 448)
-        for (row, columns, begin, end), t, c in zip(work, tiles, cost):
-            least = LEAST_WIDE_KEYS if c == 3 else LEAST_KEYS
-            pieces = 1 if whole and share is None else -(-(end - begin) // max(least, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
-            size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
-            rows, at, part = columns // G, begin, parts[row]
-            if rows == 1 and pieces == 1 and end - begin <= few:
-                solo.append((row, columns, 0, begin, end, part, 0, 0))
-                parts[row] = part + 1
-                continue
-            while at < end:
-                # cuts lie on whole blocks of the cache, so that no block is read twice
-                to = end if end - at <= size else (at + size) // BLOCK_KEYS * BLOCK_KEYS
-                (several if rows > 1 else items).extend([(row, columns, i * wide, at, to, part, 0, 0) for i in range(t)])
-                part += 1
-                at = to
-            parts[row:row + rows] = [part] * rows
+
+        def cut(most):
+            parts = [0] * self.num_rows
+            items, several, solo = [], [], []
+            for (row, columns, begin, end), t, c in zip(work, tiles, cost):
+                least = LEAST_WIDE_KEYS if c == 3 else LEAST_KEYS
+                pieces = 1 if whole and share is None else -(-(end - begin) // max(least, -(-most // (c * BLOCK_KEYS)) * BLOCK_KEYS))
+                size = -(-(-(-(end - begin) // pieces)) // BLOCK_KEYS) * BLOCK_KEYS
+                rows, at, part = columns // G, begin, parts[row]
+                if rows == 1 and pieces == 1 and end - begin <= few:
+                    solo.append((row, columns, 0, begin, end, part, 0, 0))
+                    parts[row] = part + 1
+                    continue
+                while at < end:
+                    # cuts lie on whole blocks of the cache, so that no block is read twice
+                    to = end if end - at <= size else (at + size) // BLOCK_KEYS * BLOCK_KEYS
+                    (several if rows > 1 else items).extend([(row, columns, i * wide, at, to, part, 0, 0) for i in range(t)])
+                    part += 1
+                    at = to
+                parts[row:row + rows] = [part] * rows
+            return parts, several, items, solo
+
+        parts, several, items, solo = cut(most)
+        # In float32 a few workgroups more than units cost almost a second round of them (24 rows of 32 / 4 heads of 64: 288 workgroups 16.6 us, 240 14.3).
+        groups = (len(several) + len(items) + -(-len(solo) // max(1, sharers))) * num_kv_heads
+        if float32 and units < groups <= 1.25 * units:
+            parts, several, items, solo = cut(most * 4 // 3)
         # the longest first: items of many columns take several times what those of one row do (256 rows behind 8,192 keys: the two kinds
         # spread among one another 256 us, these first 182)
         items = several + items
