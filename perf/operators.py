@@ -17,29 +17,29 @@ DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
 def listed():
     return [
         # four answers to a short prompt, a few tokens in: nothing but launches
-        dict(name="shared 4 rows of 200 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=4, dim=64, groups=1, rows=4, prefix=200, own_keys=40),
+        dict(name="shared, 4 rows of 200 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=4, dim=64, groups=1, rows=4, prefix=200, own_keys=40),
         # thirty-two answers to a prompt of one page of text
-        dict(name="shared 32 rows of 2000 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=8, dim=128, groups=1, rows=32, prefix=2000, own_keys=512),
+        dict(name="shared, 32 rows of 2000 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=8, dim=128, groups=1, rows=32, prefix=2000, own_keys=512),
         # a few answers to a long document
-        dict(name="shared 8 rows of 30000 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=8, dim=128, groups=1, rows=8, prefix=30000, own_keys=700),
+        dict(name="shared, 8 rows of 30000 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=8, dim=128, groups=1, rows=8, prefix=30000, own_keys=700),
         # eight prompts of different lengths with eight answers each
-        dict(name="shared 8 times 8 rows", op="shared", dtype="bf16", q_heads=32, kv_heads=4, dim=64, groups=8, rows=8, prefix=3500, own_keys=900),
+        dict(name="shared, 8 times 8 rows", op="shared", dtype="bf16", q_heads=32, kv_heads=4, dim=64, groups=8, rows=8, prefix=3500, own_keys=900),
         # a full batch behind one system prompt with its documents
-        dict(name="shared 256 rows of 8192 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=8, dim=128, groups=1, rows=256, prefix=8192, own_keys=1024),
+        dict(name="shared, 256 rows of 8192 keys", op="shared", dtype="bf16", q_heads=32, kv_heads=8, dim=128, groups=1, rows=256, prefix=8192, own_keys=1024),
         # the 32-bit engine: twenty-four answers
-        dict(name="shared float32 24 rows", op="shared", dtype="f32", q_heads=32, kv_heads=4, dim=64, groups=1, rows=24, prefix=1500, own_keys=100),
+        dict(name="shared, float32, 24 rows", op="shared", dtype="f32", q_heads=32, kv_heads=4, dim=64, groups=1, rows=24, prefix=1500, own_keys=100),
         # one request's next token: nothing but launches
-        dict(name="choose 1 row of 32000", op="choose", rows=1, vocab=32000, history=300, masked=0, biased=20),
+        dict(name="choose, 1 row of 32000", op="choose", rows=1, vocab=32000, history=300, masked=0, biased=20),
         # an ordinary batch, some of it under a grammar
-        dict(name="choose 32 rows of 32000", op="choose", rows=32, vocab=32000, history=2000, masked=12, biased=30),
+        dict(name="choose, 32 rows of 32000", op="choose", rows=32, vocab=32000, history=2000, masked=12, biased=30),
         # a vocabulary that is no multiple of anything, everything under a grammar
-        dict(name="choose 7 rows of 50261", op="choose", rows=7, vocab=50261, history=5000, masked=7, biased=300),
+        dict(name="choose, 7 rows of 50261", op="choose", rows=7, vocab=50261, history=5000, masked=7, biased=300),
         # a full batch of a large vocabulary
-        dict(name="choose 256 rows of 128256", op="choose", rows=256, vocab=128256, history=2000, masked=64, biased=50),
+        dict(name="choose, 256 rows of 128256", op="choose", rows=256, vocab=128256, history=2000, masked=64, biased=50),
         # logits for a caller that chooses itself
-        dict(name="adjust 8 rows of 32000", op="adjust", rows=8, vocab=32000, history=1000, masked=4, biased=10),
+        dict(name="adjust, 8 rows of 32000", op="adjust", rows=8, vocab=32000, history=1000, masked=4, biased=10),
         # and a full batch with long histories
-        dict(name="adjust 192 rows of 128256", op="adjust", rows=192, vocab=128256, history=12000, masked=96, biased=300),
+        dict(name="adjust, 192 rows of 128256", op="adjust", rows=192, vocab=128256, history=12000, masked=96, biased=300),
     ]
 
 
