@@ -29,6 +29,7 @@ class RequestCache:
     first_live: list                 # per group: first logical page still held
     state_slot: int = 0
     closed: bool = False
+    recorded: int = 0                # of its first tokens, those whose ids are where rules on logits look for them (ModelRunner.token_history)
 
 
 @dataclass

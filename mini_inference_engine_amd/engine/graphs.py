@@ -142,6 +142,7 @@ class _ScratchRequest:
     def __init__(self, num_groups: int, blocks: int):
         self.tables = [[0] * blocks for _ in range(num_groups)]
         self.state_slot = 0
+        self.recorded = 0
 
 
 class PortionGraph:

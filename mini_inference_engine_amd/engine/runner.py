@@ -128,22 +128,37 @@ class ModelRunner:
         step.earlier_tokens = self.chosen_tokens
         if self.token_history is not None:
             self.ops.record_tokens(self.token_history, step)
+            for r in rows:
+                end = r.start + len(r.tokens)
+                if r.start <= r.cache.recorded < end:
+                    r.cache.recorded = end
         return step
 
     def keep_token_history(self) -> torch.Tensor:
         """From now on every step's tokens are also written to ``token_history`` [state slots, positions]: a request's text where the
-        rules on its logits look for it (kernels.api.LogitRules).  A request has its whole text there if its first step comes later."""
+        rules on its logits look for it (kernels.api.LogitRules).  A request has its whole text there if all its tokens run later, or
+        all behind a part that ``fork`` gave it with its text; a step under penalties for one that has not is refused."""
         if self.token_history is None:
             positions = min(self.max_model_len, self.cache.max_tokens_one_request())
             self.token_history = torch.zeros((self.num_state_slots, positions), dtype=torch.int32, device=self.device)
         return self.token_history
 
-    def fork(self, rc, request_id, tokens: int):
-        """CacheManager.fork, with the text of the shared pages where the rules on logits look for it."""
+    def fork(self, rc, request_id, tokens: int, text=None):
+        """CacheManager.fork, with the text of the shared pages where the rules on logits look for it: ``text``, the request's tokens
+        from its first on, or what is kept of ``rc``'s; refused where texts are kept, but not since ``rc`` began, and none is given."""
+        shared = tokens // self.page_size * self.page_size
+        if text is not None and len(text) < shared:
+            raise ValueError(f"a text of {len(text)} tokens for the {shared} of the shared pages")
+        if self.token_history is not None and text is None and rc.recorded < shared:
+            raise ValueError(f"request {rc.request_id!r} has {rc.recorded} of its first {shared} tokens in the texts that are kept: give its text")
         new = self.cache.fork(rc, request_id, tokens)
         if self.token_history is not None:
-            shared = tokens // self.page_size * self.page_size
-            self.token_history[new.state_slot, :shared] = self.token_history[rc.state_slot, :shared]
+            row = self.token_history[new.state_slot, :shared]
+            if text is None:
+                row.copy_(self.token_history[rc.state_slot, :shared])
+            else:
+                row.copy_(torch.tensor([int(t) for t in text[:len(row)]], dtype=torch.int32))
+            new.recorded = shared
         return new
 
     def capture_decode_graphs(self, batch_sizes, verbose: bool = False, sample: bool = False) -> None:
@@ -193,7 +208,8 @@ class ModelRunner:
         travel with the step's other arrays, and in a captured step the choice is part of the graph.
 
         ``rules`` (LogitRules of the wanted rows, beside ``sampling``): the tokens are chosen under them, from logits
-        that are returned as they are.
+        that are returned as they are.  Refused for rows whose penalties look at a text that was not kept from its beginning
+        (``keep_token_history``), as far as the rules say which look (RuleInputs does).
 
         ``shared_prefix``: (rows, keys) of runs of rows, in order, that hold the same pages for their first ``keys``
         tokens (CacheManager.fork; whole pages, 0: nothing shared), for a step of single-token rows: layers that see all
@@ -202,6 +218,8 @@ class ModelRunner:
         if shared_prefix is not None:
             shared_prefix = [(int(n), int(keys)) for n, keys in shared_prefix]
             self._check_shared_prefix(rows, shared_prefix)
+        if rules is not None and rules.readers is not None and rules.history is self.token_history:
+            self._check_texts(rows, rules.readers.tolist())
         self.last_step_captured = False
         captured = (shared_prefix is None and self.graphs is not None and self.graphs.fits(len(rows)) and all(len(r.tokens) == 1 for r in rows)
                     and (sampling is None or all(len(r.want) == 1 for r in rows)))
@@ -235,6 +253,15 @@ class ModelRunner:
                 self.ops.sample(logits, step.sample_temps[:n], step.sample_seeds[:n], step.sample_counters[:n],
                                 out=self.chosen_tokens[:n], **under)
         return logits
+
+    @staticmethod
+    def _check_texts(rows, readers) -> None:
+        wanted = [r for r in rows for _ in r.want]
+        for i in readers:
+            if i < len(wanted) and wanted[i].cache.recorded < wanted[i].start:
+                rc = wanted[i].cache
+                raise ValueError(f"request {rc.request_id!r} has penalties, and {rc.recorded} of its first {wanted[i].start} tokens are in the texts "
+                                 f"that are kept (keep_token_history before they run, or ModelRunner.fork with their text)")
 
     def _plans_go_on(self, rows, runs, sampling) -> bool:
         """Whether a step with shared first parts can be captured, or is: the plans of an earlier one fit it."""

@@ -144,6 +144,7 @@ class LogitRules:
     bias_values: Any = None
     masks: Any = None
     mask_rows: Any = None
+    readers: Any = None              # a tensor on the host, where that is known: the rows whose penalties look at their text
 
 
 class KernelBackend:

@@ -94,6 +94,8 @@ class RuleInputs:
         else:
             dev = host[:len(packed)].clone()
         rules = LogitRules(history=history if "slots" in where else None)
+        if rules.history is not None:
+            rules.readers = torch.tensor([i for i, p in enumerate(params) if p.has_penalties])
         for name, (a, n) in where.items():
             t = dev[a:a + n]
             if name in ("repetition", "presence", "frequency", "bias_values"):
