@@ -68,6 +68,7 @@ class LLMEngine:
             self.runner.ranges.on = True
         self._in_flight = None             # the step whose tokens the host has not read yet
         self._reading = set()              # live requests that look at their output before each token (allowed_tokens)
+        self.failed_request = None         # whose allowed_tokens made the last step raise
         self.stop_token_ids = frozenset(self.runner.model.spec.stop_token_ids)
         self.rule_inputs = RuleInputs(self.runner.device, self.runner.vocab_size)
         if verbose:
@@ -128,6 +129,18 @@ class LLMEngine:
             self._reading.add(seq)
         return seq
 
+    def abort(self, seq: Sequence) -> bool:
+        """Ends a request, wherever it is: what it holds is free again, ``output_ids`` keeps the tokens read so far, and one that is on
+        its way is dropped.  False if it had ended already.  (``step`` does not return a request ended this way.)"""
+        if seq.status is Status.FINISHED:
+            return False
+        self._reading.discard(seq)
+        self.scheduler.drop(seq)
+        while seq.token_ids[-1] == PENDING:
+            seq.token_ids.pop()
+        seq.finish_time = time.perf_counter()
+        return True
+
     # ------------------------------------------------------------------- step
     def has_work(self) -> bool:
         return self._in_flight is not None or self.scheduler.has_work()
@@ -142,7 +155,10 @@ class LLMEngine:
         the token's value (positions, pages, the end by max_tokens or length) is decided at once; an end
         by the stop token is seen one step late, and the row already started for that request is dropped.
         While a request with ``allowed_tokens`` is there, whose next token depends on the value of its last, nothing
-        runs ahead."""
+        runs ahead.  If that function raises, or gives what is no token (or nothing, for a model without stop tokens), so does this,
+        and ``failed_request`` is the request: the step was not taken for anybody.  The next call tries the same one again; ``abort``
+        ends that request and lets the others go on."""
+        self.failed_request = None
         ahead = self.cfg.run_ahead and not self._reading
         if not ahead and self._in_flight is not None:
             finished = self.drain()
@@ -190,7 +206,11 @@ class LLMEngine:
             sampling = self.sampler.sampling_inputs(sample_seqs)
             if any(s.params.has_rules for s in sample_seqs):
                 self.rule_inputs.stop_token_ids = sorted(self.stop_token_ids)
-                rules = self.rule_inputs.make(sample_seqs, [s.num_tokens for s in sample_seqs], self.runner.token_history)
+                try:
+                    rules = self.rule_inputs.make(sample_seqs, [s.num_tokens for s in sample_seqs], self.runner.token_history)
+                except Exception:
+                    self.failed_request = self.rule_inputs.asked
+                    raise
         self.runner.forward_step(rows, sampling=sampling, **({} if rules is None else {"rules": rules}))
         self.num_steps += 1
         self.num_graph_steps += self.runner.last_step_captured
@@ -223,11 +243,7 @@ class LLMEngine:
             del seq.token_ids[place + 1:]      # a placeholder of the row started meanwhile, if any
             self._reading.discard(seq)
             seq.finish_time = now
-            if seq.status is Status.RUNNING:
-                self.scheduler.finish(seq)
-            else:                              # preempted while its last token was on its way
-                self.scheduler.waiting.remove(seq)
-                seq.status = Status.FINISHED
+            self.scheduler.drop(seq)           # (in the queue if it was preempted while its last token was on its way)
             finished.append(seq)
         return finished
 
@@ -248,9 +264,16 @@ class LLMEngine:
             params = [params or SamplingParams()] * len(prompts)
         if len(params) != len(prompts):
             raise ValueError(f"{len(prompts)} prompts but {len(params)} sampling params")
-        seqs = [self.add_request(p, sp) for p, sp in zip(prompts, params)]
-        while self.has_work():
-            self.step()
+        seqs = []
+        try:
+            for p, sp in zip(prompts, params):
+                seqs.append(self.add_request(p, sp))
+            while self.has_work():
+                self.step()
+        except Exception:
+            for s in seqs:                     # nobody waits for them any more
+                self.abort(s)
+            raise
         outs = []
         for s in seqs:
             text = None

@@ -168,3 +168,11 @@ class Scheduler:
         self.running.remove(seq)
         self.cache.close(seq.cache)
         seq.cache = None
+
+    def drop(self, seq: Sequence) -> None:
+        """``seq`` ends wherever it is, in the line or in the queue."""
+        if seq.status is Status.RUNNING:
+            self.finish(seq)
+        else:
+            self.waiting.remove(seq)
+            seq.status = Status.FINISHED

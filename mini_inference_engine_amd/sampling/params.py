@@ -19,7 +19,8 @@ class SamplingParams:
     frequency_penalty: float = 0.0  # the same, times how often they occur there
     logit_bias: dict | None = None  # token id -> what is added to its logit
     # Which tokens may come next: called with the output so far before each token, gives token ids, or None for all.  Where
-    # nothing may come, the stop tokens may.  The engine then reads every token before it starts the next step.
+    # nothing may come, the stop tokens may.  The engine then reads every token before it starts the next step, as long as such a
+    # request is there, queued or running.  What it raises, LLMEngine.step raises (LLMEngine.failed_request, LLMEngine.abort).
     allowed_tokens: Callable | None = None
 
     def __post_init__(self):

@@ -31,6 +31,7 @@ class RuleInputs:
         self.device, self.vocab_size = torch.device(device), int(vocab_size)
         self.stop_token_ids = sorted(stop_token_ids)
         self._mirrors, self._copied, self._turn = [None, None], [None, None], 0
+        self.asked = None               # the request whose allowed_tokens was last asked, until its answer is taken
 
     def _mirror(self, n: int) -> torch.Tensor:
         self._turn ^= 1
@@ -44,6 +45,7 @@ class RuleInputs:
     def make(self, seqs, lengths, history) -> LogitRules | None:
         """The rules of rows whose tokens are chosen for ``seqs``, ``lengths`` tokens of each known by then; None if nobody has any."""
         params = [s.params for s in seqs]
+        self.asked = None
         if not any(p.has_rules for p in params):
             return None
         pieces, where = [], {}
@@ -67,7 +69,10 @@ class RuleInputs:
             put("bias_values", [v for b in lists for v in b.values()], np.float32)
         masks = {}                      # row -> words
         for i, s in enumerate(seqs):
-            allowed = s.params.allowed_tokens(list(s.output_ids)) if s.params.allowed_tokens is not None else None
+            if s.params.allowed_tokens is None:
+                continue
+            self.asked = s
+            allowed = s.params.allowed_tokens(list(s.output_ids))
             if allowed is None:
                 continue
             words = mask_words(allowed, self.vocab_size)
@@ -76,6 +81,7 @@ class RuleInputs:
                     raise ValueError(f"request {s.seq_id}: no token is allowed after {s.num_output_tokens}, and the model has no stop token")
                 words = mask_words(self.stop_token_ids, self.vocab_size)
             masks[i] = words
+        self.asked = None
         if masks:
             at = {i: j for j, i in enumerate(masks)}
             put("mask_rows", [at.get(i, -1) for i in range(len(seqs))])
