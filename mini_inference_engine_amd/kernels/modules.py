@@ -8,7 +8,7 @@ from ctypes import c_double, c_float, c_int, c_long, c_void_p, py_object
 import torch
 
 from .library import register_kernel_module
-from .variants import HEAD_DIMS
+from .variants import HEAD_DIMS, SHARED_HEAD_DIMS
 
 P, I, L, F = c_void_p, c_int, c_long, c_float
 _head_variants = [(f"-DHEAD_DIM={d}",) for d in HEAD_DIMS]
@@ -178,7 +178,7 @@ register_kernel_module("prefill_attention_bf16", {
 register_kernel_module("shared_attention", {
     "mie_shared_attention_head_dim": [],
     "mie_shared_attention": [P, L, P, P, P, I, P, P, P, I, I, P, I, P, I, I, I, P, I, I, I, I, F, F, P, P],
-}, variants=_head_variants, flags=["-mllvm", "-amdgpu-mfma-vgpr-form"])
+}, variants=[(f"-DHEAD_DIM={d}",) for d in SHARED_HEAD_DIMS], flags=["-mllvm", "-amdgpu-mfma-vgpr-form"])
 # direct_calls: host code only, entry points that take tensors.
 _torch, O = os.path.dirname(torch.__file__), py_object
 register_kernel_module("direct_calls", {

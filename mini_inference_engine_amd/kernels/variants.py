@@ -6,3 +6,5 @@ up to 256) gets its variant compiled at first use.
 """
 
 HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 256)
+# shared_attention is built for every head size it takes: its layout in the LDS has a case for most of them, and the tests run each.
+SHARED_HEAD_DIMS = tuple(range(16, 257, 16))
