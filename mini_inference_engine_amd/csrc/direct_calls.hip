@@ -1,7 +1,7 @@
 // The short way from Python into kernels that a step calls with many small tensors: one call takes the tensors themselves, sees that
 // they are as the kernel needs them, makes what it returns and launches.  Host code only.  (A call of the smallest sizes, us, from Python tensor
-// by tensor with an entry point of plain numbers, and this way: choosing under rules 15.7 and 7.2, adjusting 13.9 and 5.6, attention over shared
-// keys 11.7 and 6.1; a launch is 3 of each.)
+// by tensor with an entry point of plain numbers, and this way: choosing under rules 15.7 and 7.2 to 8.1, adjusting 13.9 and 5.4 to 5.6, attention over
+// shared keys 11.7 and 6.1 to 6.4; a launch is 3 of each.)
 //
 // Every entry point returns a tensor, or None where something is not as it has to be or is none of the usual cases: the caller then goes
 // the long way, which says what is wrong.  Loaded with Python's lock held throughout.

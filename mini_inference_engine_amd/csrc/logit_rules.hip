@@ -13,11 +13,13 @@
 // the slice's logits, asked for before the text is read, past those words.  Every slice reads the row's whole text; it comes from the L2 for
 // all slices but one.  Biases are settled after that, the last of a token's entries first.
 //
-// What bounds it, of what a call cannot do without (MI355X): 256 rows of 128,256 with texts of 700 to 2,000 tokens chosen in 43 us, where the 134 MB
-// of logits take 26 at the rate of a large copy: reading alone, in this division, takes 25 with the join of the slices, texts 7.5, biases 5, masks 1 and
-// noise on a quarter of the rows 6, all of them vector instructions, which keep the units busy for 65 % of the time.  192 rows with texts of 4,000 to
-// 12,000 adjusted in 41 us, 40 for their 205 MB; results are stored past the L2s, where they would push out what the slices share (49 us otherwise;
-// logits read that way: 46.5, and choosing 44.5).  Tried and slower (us of the two, where the present form took 52 and 53): slices of 8,192 on 512
+// What bounds it, of what a call cannot do without (MI355X; "the same" is one call's inputs again and again, "others" several calls' in turn): 256 rows
+// of 128,256 with texts of 700 to 2,000 tokens chosen in 43 us of the same, 44 to 46 of others, where the 134 MB of logits take 19 at the rate of a
+// kernel that only reads.  Reading alone, in this division, takes 25 with the join of the slices, texts 7.5, biases 5, masks 1 and noise on a quarter
+// of the rows 6, all of them vector instructions, which keep the units busy for 65 % of the time.  192 rows with texts of 4,000 to 12,000 adjusted in
+// 42 us of the same, 47 to 49 of others, where their 205 MB take 40 at the rate of a large copy; results are stored past the L2s, where they would push
+// out what the slices share (49 of the same and 50 of others otherwise; logits read that way: 46.5 and, choosing, 44.5 of the same).  Recording a step's
+// tokens is a call of 8 us, of 1 token or 2,048: the host's.  Tried and slower (us of the two, where the present form took 52 and 53): slices of 8,192 on 512
 // threads (62 and 59) or on 256 (62 and 59), of 6,144 (52.5 and 53); tokens with a word gathered in a list and taken by themselves (64 and 57); a bound
 // on the noise by one logarithm before the exact two (63); text and list asked for before the words are cleared (62 and 79).  An entry of the list that
 // claims its token before the text is counted saves three barriers and 1 %.

@@ -20,9 +20,9 @@
 //   bytes two waves take every second 32: their LDS then leaves room for a second workgroup (150 rows of 16 / 2 heads of 256 with up to 308 keys
 //   25.4 -> 16.7 us).  Where such items are many and short, each of these waves has one to itself, and nothing is joined in the LDS.
 //
-// What bounds it (MI355X).  256 rows of 32 / 8 heads of 128 behind 8,192 shared keys with 1 to 1,024 of their own, 107 to 116 us with the join: the 540 MB
-// of own keys alone take 110 (about the rate of a large copy), the 34 GFLOP over shared keys alone 67, hidden behind them as long as the own keys'
-// waves, which wait for no other wave, share the units (with four waves a row 131 to 141).  Many columns alone are a chain of LDS reads, products and
+// What bounds it (MI355X).  256 rows of 32 / 8 heads of 128 behind 8,192 shared keys with 1 to 1,024 of their own, 106 to 111 us with the join.  In the same
+// run the 540 MB of own keys alone take 88 to 92 (5.9 TB/s), the 34 GFLOP over shared keys alone 63 to 66, for the most part hidden behind them as long as
+// the own keys' waves, which wait for no other wave, share the units (with four waves a row 131 to 141).  Many columns alone are a chain of LDS reads, products and
 // softmax: of 1,024 keys of 128 a workgroup of 128 columns takes 34 us by itself, two on a unit 51.  8 rows behind 30,000 keys 32.5 us for 134 MB (4.1
 // TB/s).  32 rows behind 2,000 keys 18 to 19 us, 4 of them the join: a workgroup's first loads, last stores and one stage take 7 us.
 #include "attention_bf16_common.hpp"

@@ -84,7 +84,7 @@ class StepContext:
 
     def prefix_plan(self, ops, num_q_heads: int, num_kv_heads: int, head_dim: int):
         """The backend's plan of ``shared_prefix`` for layers with such heads, made by the first of them: for contexts that are a
-        little longer, so that the steps that follow with the same runs of rows find it made (256 rows: 0.5 ms on the host)."""
+        little longer, so that the steps that follow with the same runs of rows find it made (256 rows: 0.25 ms on the host, 0.75 on a slower one)."""
         key = (num_q_heads, num_kv_heads, head_dim)
         plan = self.prefix_plans.get(key)
         if plan is None:

@@ -135,7 +135,7 @@ class ModelRunner:
         return step
 
     def keep_token_history(self) -> torch.Tensor:
-        """From now on every step's tokens are also written to ``token_history`` [state slots, positions]: a request's text where the
+        """From now on, for as long as the runner lives, every step's tokens are also written to ``token_history`` [state slots, positions]: a request's text where the
         rules on its logits look for it (kernels.api.LogitRules).  A request has its whole text there if all its tokens run later, or
         all behind a part that ``fork`` gave it with its text; a step under penalties for one that has not is refused."""
         if self.token_history is None:

@@ -3,7 +3,9 @@
 A step of single-token rows falls into runs of rows; the rows of a run share their first ``keys`` keys, read through the block
 table of the run's first row.  The plan cuts the step into items, each one workgroup a kv head (csrc/shared_attention.hip):
 columns (query heads of rows) x keys, so that all items take about the same time and there are as many as compute units; the
-short items of single rows come last and get a wave each.
+short items of single rows come last and get a wave each.  Making one is host work, several times what the attention it plans takes (40 us for 4 rows,
+81 for 32, 135 for 8 runs of 8, 247 for 256, the copy asked for but not waited for; three times that on slower hosts): it pays over a step's layers
+and the steps that go on with it.
 An item leaves a partial result for each of its columns; a row's partial results are its items in order of keys.
 """
 from __future__ import annotations
@@ -18,7 +20,8 @@ BLOCK_KEYS = 32
 LEAST_KEYS = 64         # of a cut: an item's start and its partial result cost about as much
 START = 500             # what a workgroup's start and end cost, in keys of an item of up to 16 columns
 LEAST_WIDE_KEYS = 192   # the same of items of more than 64 columns in bfloat16, whose partial results are the larger (32 rows behind 2,000
-                        # keys in such items: cuts of 64 keys 22 us, of 128 18.7, of 192 17.1, of 256 18.8)
+                        # keys in such items: cuts of 64 keys 22 us, of 128 18.7, of 192 17.1, of 256 18.8; fourteen drawn shapes whose cuts
+                        # this moves, 5 to 146 rows behind 1,000 to 11,600 keys, in geometric mean of 64 to 192 18.5, of 256 17.4, of 320 17.7)
 
 
 def _sharers(head_dim: int, float32: bool) -> int:
@@ -119,7 +122,8 @@ class SharedPrefixPlan:
             return parts, several, items, solo
 
         parts, several, items, solo = cut(most)
-        # In float32 a few workgroups more than units cost almost a second round of them (24 rows of 32 / 4 heads of 64: 288 workgroups 16.6 us, 240 14.3).
+        # In float32 a few workgroups more than units cost almost a second round of them (24 rows of 32 / 4 heads of 64: 288 workgroups 16.6 us, 240 14.3;
+        # sixteen drawn shapes of heads of 16 to 256 that this cuts otherwise, in geometric mean 20.6 and 19.3, eleven of them faster, five up to 16 % slower).
         groups = (len(several) + len(items) + -(-len(solo) // max(1, sharers))) * num_kv_heads
         if float32 and units < groups <= 1.25 * units:
             parts, several, items, solo = cut(most * 4 // 3)
